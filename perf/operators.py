@@ -141,7 +141,7 @@ def _prepare_prefix(case, seed):
     for t in new:
         cu.append(cu[-1] + t)
     return dict(kind="prefix", case=case, q=q, keys=store[0], values=store[1], table=table.cuda(), cu_q=ints(cu),
-                ctx_len=ints([P + b for b in behind]), prefix_len=ints([P] * n),
+                ctx_len=ints([P + b for b in behind]), prefix_len=ints([P] * case["groups"]),
                 group_off=ints([g * case["members"] for g in range(case["groups"] + 1)]), single=case["tokens"] == 1,
                 heads=s["heads"], kv_heads=s["kv_heads"], dim=d, scale=d ** -0.5, out=torch.empty_like(q))
 
