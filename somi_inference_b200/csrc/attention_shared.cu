@@ -1,0 +1,300 @@
+// Attention of a batch whose requests share their first positions in groups, for any type and head size
+// (shared_prefix.cuh says how the work is cut), and the kernel that joins the parts.
+//
+// A CTA holds up to 64 query rows (the query heads of a key/value head, of as many tokens as fit) in
+// shared memory as float32 and walks through its pieces in tiles of 64 keys: scores and outputs by
+// float32 FMAs, four rows by four columns a thread, the softmax online in float32, base 2.  It is the
+// path of float32 and of head sizes and pages that the tensor-core kernel does not take.
+#include "mma.cuh"
+#include "shared_prefix.cuh"
+#include "vec4.cuh"
+
+namespace somi {
+namespace shp {
+
+constexpr int kRows = 64, kKeys = 64, kThreads = 256;
+
+// HD: the head size rounded up to 64, 128 or 256; d: the head size (a multiple of 16)
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads)
+shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stride, const T* __restrict__ keys,
+                        const T* __restrict__ values, int d, float scale_log2e, Note* __restrict__ notes,
+                        unsigned* __restrict__ header, Parts parts) {
+    constexpr int LD = HD + 4;                       // floats of a row: 16-byte reads of 8 rows meet no bank twice
+    constexpr int LP = kKeys + 4;
+    constexpr int COLS = HD / 16;                    // output columns of a thread
+    extern __shared__ __align__(16) float smem[];
+    float* Qs = smem;                                // [kRows][LD]
+    float* KV = Qs + kRows * LD;                     // [kKeys][LD], keys, then values
+    float* Ps = KV + kKeys * LD;                     // [kRows][LP]
+    __shared__ RangeScratch scratch;
+
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const Range range = find_range<kThreads>(b, scratch);     // [descriptor]
+    pdl_wait();
+    write_notes<kThreads>(b, scratch, range.total, notes, header);
+
+    Walk walk(b, range);
+    Piece p;
+    while (walk.next(b, p)) {
+        const int rows = p.tokens * b.per;
+        __syncthreads();
+        for (int i = tid; i < kRows * (HD / 4); i += kThreads) {
+            const int row = i / (HD / 4), c = (i % (HD / 4)) * 4;
+            F4 v{{0.f, 0.f, 0.f, 0.f}};
+            if (row < rows && c < d) {
+                const int token = p.token0 + row / b.per, head = p.kvh * b.per + row % b.per;
+                v = load4(q + token * q_stride + static_cast<size_t>(head) * d + c);
+            }
+            store4(Qs + row * LD + c, v);
+        }
+        float m[4], l[4], o[4][COLS];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) o[i][c] = 0.f;
+        }
+        int last[4];                                 // the last key that a row sees
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = ty * 4 + i;
+            const int t = row / b.per + (p.token0 - p.x.first);
+            last[i] = row < rows ? min(p.x.key_hi - 1, p.x.pos0 + t) : -1;
+        }
+        const int kb0 = p.x.base(b);
+        const int* table = b.block_table + static_cast<size_t>(p.x.table) * b.bt_stride;
+        // one tile of keys or values; what lies outside the piece's keys, or on no page, becomes zeros
+        auto load_tile = [&](const T* __restrict__ from, int k0) {
+            for (int i = tid; i < kKeys * (HD / 4); i += kThreads) {
+                const int key = i / (HD / 4), c = (i % (HD / 4)) * 4, pos = k0 + key;
+                F4 v{{0.f, 0.f, 0.f, 0.f}};
+                if (c < d && pos >= p.x.key_lo && pos < p.x.key_hi) {
+                    const int page = table[pos / b.page_size];
+                    if (static_cast<unsigned>(page) < static_cast<unsigned>(b.num_pages))
+                        v = load4(from + ((static_cast<size_t>(page) * b.nkv + p.kvh) * b.page_size + pos % b.page_size) * d + c);
+                }
+                store4(KV + key * LD + c, v);
+            }
+        };
+        for (int u = p.unit0; u < p.unit1; ++u) {
+            const int k0 = kb0 + u * p.x.unit;
+            __syncthreads();
+            load_tile(keys, k0);
+            __syncthreads();
+            float s[4][4] = {};
+            for (int c = 0; c < HD; c += 4) {
+                F4 a[4], k[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = load4(Qs + (ty * 4 + i) * LD + c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) k[j] = load4(KV + (tx + 16 * j) * LD + c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[i][j] = fmaf(a[i].v[e], k[j].v[e], s[i][j]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int pos = k0 + tx + 16 * j;
+                    s[i][j] = pos >= p.x.key_lo && pos <= last[i] ? s[i][j] * scale_log2e : -INFINITY;
+                    top = fmaxf(top, s[i][j]);
+                }
+#pragma unroll
+                for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                const float now = fmaxf(m[i], top);
+                const float ref = now == -INFINITY ? 0.f : now;
+                const float keep = exp2f(m[i] - ref);
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float w = exp2f(s[i][j] - ref);
+                    sum += w;
+                    Ps[(ty * 4 + i) * LP + tx + 16 * j] = w;
+                }
+#pragma unroll
+                for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                l[i] = l[i] * keep + sum;
+                m[i] = now;
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) o[i][c] *= keep;
+            }
+            __syncthreads();                         // all threads have read the keys
+            load_tile(values, k0);
+            __syncthreads();
+            // (a value that a row does not see stays out of its sum even if it is infinite)
+            const bool all_seen = k0 + kKeys - 1 <= p.x.pos0;
+            for (int j = 0; j < kKeys; j += 4) {
+                F4 w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = load4(Ps + (ty * 4 + i) * LP + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int c = 0; c < COLS; ++c) {
+                        const float v = KV[(j + e) * LD + tx + 16 * c];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (all_seen || k0 + j + e <= last[i]) o[i][c] = fmaf(w[i].v[e], v, o[i][c]);
+                    }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = ty * 4 + i;
+            if (row >= rows) continue;
+            const size_t at = part_row(b, p.x.pos0 == 0x3fffffff, p.first, blockIdx.x, kRows, p.token0 + row / b.per,
+                                       p.kvh * b.per + row % b.per, row);
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+                if (tx + 16 * c < d) parts.o[at * d + tx + 16 * c] = o[i][c];
+            if (tx == 0) parts.ml[at] = make_float2(m[i], l[i]);
+        }
+    }
+}
+
+constexpr int kMergeWarps = 8;
+
+// A warp per (token, head).
+template <typename T>
+__global__ void __launch_bounds__(kMergeWarps * 32)
+shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const unsigned* __restrict__ header, Parts parts,
+                    int ctas, int block_rows, T* __restrict__ out) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const long long row = static_cast<long long>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
+    if (row >= static_cast<long long>(b.T) * b.nq) return;
+    const int t = static_cast<int>(row / b.nq), h = static_cast<int>(row % b.nq), kvh = h / b.per;
+    if (b.cu_q && (t < b.cu_q[0] || t >= b.cu_q[b.R])) return;     // a row of no request stays as it was
+    const unsigned total = header[0];
+    if (total == 0) return;
+    const Shares shares(total, ctas);
+    constexpr int COLS = 4;                          // of four columns a lane reads at a time: head sizes to 512
+    float m = -INFINITY, l = 0.f;
+    F4 o[COLS / 2];
+#pragma unroll
+    for (int c = 0; c < COLS / 2; ++c) o[c] = F4{{0.f, 0.f, 0.f, 0.f}};
+    const Note own = notes[b.T + t];
+    for (int which = 0; which < 2; ++which) {        // the prefix, then the request's own keys
+        if (which == 0 && !(own.place >> 30 & 1)) continue;
+        Note n = which == 0 ? notes[t] : own;
+        n.place &= (1 << 30) - 1;
+        if (n.units <= 0) continue;
+        const unsigned begin = n.begin + static_cast<unsigned>(kvh) * n.cost, end = begin + n.cost;
+        // (what no request of a consistent call leads to)
+        if (n.cost != n.units + kOverhead || end > total || end < begin || n.place >= b.item_tokens) continue;
+        for (unsigned cta = shares.cta_of(begin); cta < static_cast<unsigned>(ctas); ++cta) {
+            const unsigned c0 = shares.begin(cta), c1 = shares.begin(cta + 1);
+            if (c0 >= end) break;
+            const unsigned o0 = c0 > begin ? c0 - begin : 0, o1 = min(c1, end) - begin;
+            if (o1 <= kOverhead || o1 <= o0) continue;              // it had only the item's fixed cost
+            const size_t at = part_row(b, which == 0, o0 == 0, cta, block_rows, t, h, n.place * b.per + h % b.per);
+            const float2 ml = parts.ml[at];
+            const float now = fmaxf(m, ml.x);
+            if (now == -INFINITY) continue;          // none of its keys is seen
+            const float keep = exp2f(m - now), w = exp2f(ml.x - now);
+            l = l * keep + ml.y * w;
+            m = now;
+#pragma unroll
+            for (int c = 0; c < COLS / 2; ++c) {
+                const int col = (c * 32 + lane) * 4;
+                if (col < d) {
+                    const F4 v = load4(parts.o + at * d + col);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[c].v[e] = fmaf(v.v[e], w, o[c].v[e] * keep);
+                }
+            }
+        }
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+    for (int c = 0; c < COLS / 2; ++c) {
+        const int col = (c * 32 + lane) * 4;
+        if (col < d) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c].v[e] *= inv;
+            store4(out + row * d + col, o[c]);
+        }
+    }
+}
+
+template <typename T, int HD>
+int launch_shared(const Batch& b, const void* q, long long q_stride, const void* keys, const void* values, int d, float scale,
+                  Note* notes, unsigned* header, Parts parts, int ctas, cudaStream_t stream) {
+    constexpr int smem = (kRows * (HD + 4) + kKeys * (HD + 4) + kRows * (kKeys + 4)) * 4;
+    allow_smem<shared_attention_kernel<T, HD>>(smem);
+    return launch_pdl(shared_attention_kernel<T, HD>, dim3(ctas), dim3(kThreads), smem, stream, b,
+                      static_cast<const T*>(q), q_stride, static_cast<const T*>(keys), static_cast<const T*>(values), d,
+                      scale * 1.4426950408889634f, notes, header, parts);
+}
+
+}  // namespace shp
+}  // namespace somi
+
+using namespace somi;
+using namespace somi::shp;
+
+// CTAs of a call (whichever kernel), and the rows of one CTA's continuation: what a caller needs for the workspace.
+static int shared_ctas(int hd, int per_sm) {
+    int device = 0, sms = 0;
+    cudaGetDevice(&device);
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) return 0;
+    return sms * per_sm;
+}
+SOMI_API int somi_shared_attention_ctas(int hd) { return shared_ctas(hd, hd <= 64 ? 4 : hd <= 128 ? 2 : 1); }
+SOMI_API int somi_shared_attention_block_rows() { return kRows; }
+
+// Bytes of workspace: notes, the header, maxima and sums, outputs.
+static long long workspace_bytes(long long T, int nq, int hd, int ctas, int block_rows) {
+    const long long rows = 2 * T * nq + static_cast<long long>(ctas) * block_rows;
+    return 2 * T * static_cast<long long>(sizeof(Note)) + 16 + rows * 8 + rows * hd * 4;
+}
+
+// qkv [T, >= nq hd] (rows `q_stride` elements apart), keys and values [num_pages, nkv, page_size, hd], block_table
+// [R, bt_stride], cu_q [R + 1] or null (then T = R, one token per request), ctx_len [R], group_off [G + 1], prefix_len [G];
+// `out` [T, nq hd].  Refuses what it cannot take; the lengths are read on the device.
+SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_stride, const void* keys, const void* values,
+                                   const int* block_table, int bt_stride, const int* cu_q, const int* ctx_len,
+                                   const int* prefix_len, const int* group_off, int T, int R, int G, int nq, int nkv, int hd,
+                                   int page_size, int num_pages, float scale, void* workspace, long long bytes, int ctas,
+                                   void* out, cudaStream_t stream) {
+    if (T <= 0 || R <= 0) return 0;
+    if (nkv <= 0 || nq <= 0 || nq % nkv || nq / nkv > kRows || hd % 16 || hd < 16 || hd > 256 || G < 0 || bt_stride <= 0 ||
+        page_size <= 0 || num_pages <= 0 || ctas <= 0 || static_cast<long long>(R) + G > kMaxEntries ||
+        static_cast<long long>(R) + G > static_cast<long long>(ctas) * kOwned || (!cu_q && T != R))
+        return SOMI_ERR_UNSUPPORTED;
+    const long long span = static_cast<long long>(bt_stride) * page_size;
+    const int item_tokens = kRows / (nq / nkv);
+    const long long items = (R + static_cast<long long>(G) + 2 * (T / item_tokens + 1ll)) * nkv;
+    if (span > 0x3fff0000ll || items * (span / kKeys + 3) > 0x7fffffffll || (static_cast<long long>(T) * nq + 7) / 8 > 0x7fffffffll)
+        return SOMI_ERR_UNSUPPORTED;
+    if (bytes < workspace_bytes(T, nq, hd, ctas, kRows)) return SOMI_ERR_SCRATCH_TOO_SMALL;
+    Batch b{cu_q, ctx_len, prefix_len, group_off, block_table, bt_stride, R, G, T, nq, nkv, nq / nkv, page_size, num_pages,
+            item_tokens, item_tokens, kKeys, kKeys, kKeys};
+    char* at = static_cast<char*>(workspace);
+    Note* notes = reinterpret_cast<Note*>(at);
+    unsigned* header = reinterpret_cast<unsigned*>(at + 2ll * T * sizeof(Note));
+    const long long rows = 2ll * T * nq + static_cast<long long>(ctas) * kRows;
+    Parts parts;
+    parts.o = reinterpret_cast<float*>(header + 4);
+    parts.ml = reinterpret_cast<float2*>(parts.o + rows * hd);
+    const auto launch = [&](auto kind) {
+        using E = decltype(kind);
+        int rc = hd <= 64    ? launch_shared<E, 64>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
+                 : hd <= 128 ? launch_shared<E, 128>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
+                             : launch_shared<E, 256>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream);
+        if (rc) return rc;
+        const long long out_rows = static_cast<long long>(T) * nq;
+        return launch_pdl(shared_merge_kernel<E>, dim3(static_cast<unsigned>((out_rows + kMergeWarps - 1) / kMergeWarps)),
+                          dim3(kMergeWarps * 32), 0, stream, b, hd, notes, header, parts, ctas, kRows, static_cast<E*>(out));
+    };
+    return dtype == SOMI_F32 ? launch(float{}) : dtype == SOMI_BF16 ? launch(__nv_bfloat16{}) : SOMI_ERR_UNSUPPORTED;
+}

@@ -112,6 +112,10 @@ class CudaOps:
         self.lib.somi_decode_ring_chunks.restype = None
         self.use_tma_prefill = True
         self._gemm_maps: dict = {}
+        self._shared_plans: dict = {}      # (type, head size) -> CTAs and rows of a block of attention over shared prefixes
+        self._shared_attention = self.lib.somi_shared_attention
+        p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+        self._shared_attention.argtypes = [p, i, n, p, p, p, i, p, p, p, p, i, i, i, i, i, i, i, i, ctypes.c_float, p, n, i, p, p]
         self.use_skinny_gemm = True
         self.skinny_max_tokens = int(self.lib.somi_skinny_gemm_max_tokens())
         self._retired: list = []
@@ -654,6 +658,64 @@ class CudaOps:
                 self.head_gate_mul(out[first:last], gate[first:last], nq)
             else:
                 self.sigmoid_gate_mul(out[first:last], gate[first:last])
+
+    def shared_prefix_attention(self, qkv, kcache, vcache, block_table, ctx_len, prefix_len, group_off, nq: int,
+                                nkv: int, hd: int, scale: float, out, cu_q=None) -> None:
+        """Attention over the cache of a batch whose requests share their first positions in groups: the
+        shared keys and values are read, and multiplied with all rows of a group, once a group.
+
+        `qkv` [T, width] holds the queries in its first nq * hd columns (rows may lie further apart);
+        request r's tokens are rows cu_q[r] .. cu_q[r + 1] (`cu_q` None: one token per request) and
+        continue from ctx_len[r] cached positions; its keys and values, those of its new tokens among
+        them, lie in the pages of block_table[r] (`kcache`, `vcache` [pages, nkv, page size, hd]).  Group g
+        is the neighbouring requests group_off[g] .. group_off[g + 1], which all have the same first
+        prefix_len[g] positions (any number up to the least of their ctx_len); these are read through the
+        first member's table.  A request that is in no group shares nothing.  Every token sees its request's
+        positions up to its own.  Rows that belong to no request, in front of cu_q[0] or from cu_q[R] on, are left as they are.
+
+        All lengths are read on the device: a captured call may be replayed with others (of the same
+        numbers of requests, groups and tokens).  bfloat16 or float32, head sizes in multiples of 16 up to
+        256, at most 64 query heads a key/value head and 8,192 requests and groups.
+        """
+        if not (qkv.dim() == 2 and qkv.stride(1) == 1 and tuple(out.shape) == (qkv.shape[0], nq * hd)
+                and qkv.shape[1] >= nq * hd and out.dtype == kcache.dtype == vcache.dtype == qkv.dtype):
+            raise KernelError("queries are [T, width >= heads * head size] with contiguous rows, the output [T, heads * head "
+                              "size], both of the cache's dtype")
+        ints = (block_table, ctx_len, prefix_len, group_off) + (() if cu_q is None else (cu_q,))
+        _check(out, kcache, vcache, *ints)
+        if not qkv.is_cuda or any(t.device != out.device for t in (qkv, kcache, vcache, *ints)) \
+                or out.device.index != self._device_index or torch.cuda.current_device() != self._device_index:
+            raise KernelError("shared_prefix_attention: all tensors on the kernel table's device, which is the current one")
+        T, R, G = qkv.shape[0], ctx_len.numel(), prefix_len.numel()
+        if any(t.dtype != torch.int32 for t in ints) or kcache.shape != vcache.shape or kcache.dim() != 4 \
+                or tuple(kcache.shape[1::2]) != (nkv, hd) or block_table.dim() != 2 or block_table.shape[0] != R \
+                or group_off.numel() != G + 1 or (cu_q is not None and cu_q.numel() != R + 1) or (cu_q is None and T != R):
+            raise KernelError("a shared batch has int32 block_table [R, width], ctx_len [R], prefix_len [G], group_off [G + 1] "
+                              "and cu_q [R + 1] (without it T = R tokens), and caches [pages, kv heads, page size, head size]")
+        self.check_attention_geometry(nq, nkv, hd)
+        pages, page_size = kcache.shape[0], kcache.shape[2]
+        if (qkv.stride(0) * qkv.element_size()) % 16 or qkv.data_ptr() % 16 or out.data_ptr() % 16 \
+                or kcache.data_ptr() % 16 or vcache.data_ptr() % 16:
+            raise KernelError("query rows, outputs and caches begin on 16-byte boundaries")
+        if T == 0 or R == 0:
+            return
+        code = _code(qkv)
+        plan = self._shared_plans.get((code, hd))
+        if plan is None:
+            plan = self._shared_plans[(code, hd)] = (int(self.lib.somi_shared_attention_ctas(ctypes.c_int(hd))),
+                                                     int(self.lib.somi_shared_attention_block_rows()))
+        ctas, block_rows = plan
+        rows = 2 * T * nq + ctas * block_rows
+        work = torch.empty(32 * T + 16 + rows * (8 + 4 * hd), dtype=torch.uint8, device=qkv.device)
+        rc = self._shared_attention(
+            qkv.data_ptr(), code, qkv.stride(0), kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(),
+            block_table.shape[1], None if cu_q is None else cu_q.data_ptr(), ctx_len.data_ptr(), prefix_len.data_ptr(),
+            group_off.data_ptr(), T, R, G, nq, nkv, hd, page_size, pages, scale, work.data_ptr(), work.numel(), ctas,
+            out.data_ptr(), self._stream())
+        self._done(rc, "shared_prefix_attention")
+        self.launches += 1
+        if trace.active():
+            trace.note("attention_shared", 2 * T * nq * hd * qkv.element_size(), detail="with merge; without keys and values")
 
     def two_map_attention(self, qkv, kcache, vcache, batch, group, nq, nkv, d, vd, scale, window, keep,
                           factor: float, eps: float, gain: float, gate, out, storage=None) -> None:

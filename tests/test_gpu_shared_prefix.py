@@ -1,0 +1,148 @@
+"""Attention over shared prefixes (`CudaOps.shared_prefix_attention`) against 64 bits."""
+
+import pytest
+import torch
+
+from tests.shared_prefix_case import Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from somi_inference_b200.ops import cuda_ops
+    return cuda_ops()
+
+
+def ones(*own):
+    return [(n, 1) for n in own]
+
+
+def sums(case):
+    return "bfloat16" if case.dtype == torch.bfloat16 else "float32"
+
+
+HEADS = [(14, 2, 64), (28, 4, 128), (4, 4, 128), (8, 1, 64), (5, 1, 48), (6, 2, 16), (4, 2, 256), (16, 1, 128), (3, 1, 96)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nq,nkv,hd", HEADS)
+def test_single_tokens(ops, nq, nkv, hd, dtype):
+    """Two groups of unequal size and a request by itself; own positions from none to several tiles."""
+    case = Case(nq, nkv, hd, 16, [(160, ones(0, 1, 37, 300)), (400, ones(9, 129))], dtype, seed=hd + nq, loose=[(45, 1)])
+    case.check(case.call(ops), sums(case))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page", [1, 8, 16, 24, 64, 128, 256])
+@pytest.mark.parametrize("prefix", [1, 16, 127, 128, 129, 500])
+def test_pages_and_prefixes_that_end_inside_a_page(ops, page, prefix, dtype):
+    case = Case(8, 2, 64, page, [(prefix, ones(0, 3, 70))], dtype, seed=page + prefix)
+    case.check(case.call(ops), sums(case))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nq,nkv,hd", [(28, 4, 128), (14, 2, 64), (3, 1, 96)])
+def test_portions_of_any_length(ops, nq, nkv, hd, dtype):
+    """One token to several tiles, behind a prefix, with and without positions of their own, in any order."""
+    case = Case(nq, nkv, hd, 16, [(336, [(0, 5), (17, 1), (0, 131), (64, 64), (130, 18), (3, 290)]), (64, [(0, 1)])], dtype,
+                seed=3, loose=[(0, 33), (0, 1), (200, 2)])
+    case.check(case.call(ops), sums(case))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_without_a_prefix_and_without_groups(ops, dtype):
+    case = Case(8, 2, 128, 16, [(0, ones(0, 5, 200)), (128, [])], dtype, seed=4, loose=[(300, 1), (0, 1)])
+    case.check(case.call(ops), sums(case))
+    case = Case(8, 2, 128, 16, [], dtype, seed=5, loose=[(300, 1), (0, 3)])
+    case.check(case.call(ops), sums(case))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_of_no_request_and_rows_that_lie_apart(ops, dtype):
+    case = Case(14, 2, 64, 16, [(96, [(4, 3), (0, 1), (30, 9)])], dtype, seed=6, extra_columns=264, rows_in_front=2, rows_behind=5)
+    case.check(case.call(ops), sums(case))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_requests_and_groups(ops, dtype):
+    """More entries than a block has threads."""
+    groups = [(16 * (1 + g % 3), ones(*[(7 * g + i) % 23 for i in range(1 + g % 4)])) for g in range(250)]
+    case = Case(4, 2, 64, 16, groups, dtype, seed=7, loose=[(i % 50, 1) for i in range(100)])
+    case.check(case.call(ops), sums(case))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_long_prefix_in_many_parts(ops, dtype):
+    case = Case(2, 1, 64, 16, [(20000, ones(0, 100))], dtype, seed=8)
+    case.check(case.call(ops), sums(case))
+
+
+def test_far_apart_scores(ops):
+    """The largest score lies in the prefix for one row and among its own keys for another, hundreds above the rest."""
+    for dtype in (torch.bfloat16, torch.float32):
+        case = Case(8, 2, 128, 16, [(512, ones(200, 130, 1))], dtype, seed=9, scale=3.0)
+        case.check(case.call(ops), sums(case))
+
+
+def test_equal_calls_give_equal_bits_and_other_streams(ops):
+    case = Case(28, 4, 128, 16, [(2048, ones(*range(0, 160, 9)))], torch.bfloat16, seed=10)
+    first = case.call(ops).clone()
+    side = torch.cuda.Stream()
+    outs = []
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        for _ in range(3):
+            outs.append(case.call(ops, out=torch.empty_like(case.out)))
+    for _ in range(3):
+        outs.append(case.call(ops, out=torch.empty_like(case.out)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, o) for o in outs)
+
+
+def test_captured_calls_with_other_lengths(ops):
+    """Two graphs of the same ops, replayed in turn, with lengths and tables that change between replays."""
+    a = Case(14, 2, 64, 16, [(320, ones(0, 40, 7))], torch.bfloat16, seed=11)
+    b = Case(14, 2, 64, 16, [(48, ones(300, 2, 150))], torch.bfloat16, seed=12)
+    assert a.qkv.shape == b.qkv.shape
+    width = max(a.table.shape[1], b.table.shape[1])
+    pages = max(a.keys.shape[0], b.keys.shape[0])
+    hold = {n: torch.zeros_like(getattr(a, n)) for n in ("qkv", "ctx_len", "prefix_len", "group_off", "out")}
+    hold["table"] = torch.full((3, width), -1, dtype=torch.int32, device="cuda")
+    hold["keys"] = torch.zeros((pages, *a.keys.shape[1:]), dtype=a.dtype, device="cuda")
+    hold["values"] = torch.zeros_like(hold["keys"])
+
+    def load(c):
+        for n in ("qkv", "ctx_len", "prefix_len", "group_off"):
+            hold[n].copy_(getattr(c, n))
+        hold["table"][:, :c.table.shape[1]] = c.table
+        hold["keys"][:c.keys.shape[0]] = c.keys
+        hold["values"][:c.keys.shape[0]] = c.values
+
+    def call():
+        ops.shared_prefix_attention(hold["qkv"], hold["keys"], hold["values"], hold["table"], hold["ctx_len"],
+                                    hold["prefix_len"], hold["group_off"], 14, 2, 64, a.scale, hold["out"])
+
+    load(a)
+    call()
+    graphs = []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call()
+    for i, c in enumerate((b, a, a, b)):
+        load(c)
+        hold["out"].zero_()
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        c.check(hold["out"], "bfloat16")
+
+
+def test_no_rows_is_no_launch(ops):
+    before = ops.launches
+    case = Case(4, 2, 64, 16, [(16, ones(1))], torch.float32)
+    empty = torch.empty((0, 256), device="cuda")
+    ints = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.shared_prefix_attention(empty, case.keys, case.values, case.table[:0], ints[:0], ints[:0], ints, 4, 2, 64, 1.0,
+                                torch.empty((0, 256), device="cuda"))
+    assert ops.launches == before

@@ -1,0 +1,88 @@
+"""What `CudaOps.shared_prefix_attention` refuses before it launches anything, without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+from somi_inference_b200.ops import KernelError, cuda
+from tests.test_kernel_table import OnDevice
+
+
+def on_device(t):
+    return t.as_subclass(OnDevice)
+
+
+@pytest.fixture
+def ops(monkeypatch):
+    """A kernel table over CPU tensors whose launcher notes its calls."""
+    table = cuda.CudaOps.__new__(cuda.CudaOps)
+    table.launches, table._device_index, table.calls = 0, None, []
+    table._shared_plans = {}
+    table.lib = type("Library", (), {})()
+    table.lib.somi_shared_attention_ctas = lambda hd: 148
+    table.lib.somi_shared_attention_block_rows = lambda: 64
+    table._shared_attention = lambda *a: table.calls.append(a) or 0
+    table._stream = lambda: ctypes.c_void_p(0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    return table
+
+
+def arguments(**changed):
+    T, R, G, nq, nkv, hd, page = 3, 3, 1, 4, 2, 64, 16
+    a = dict(qkv=torch.zeros(T, nq * hd), kcache=torch.zeros(9, nkv, page, hd), vcache=torch.zeros(9, nkv, page, hd),
+             block_table=torch.zeros(R, 5, dtype=torch.int32), ctx_len=torch.zeros(R, dtype=torch.int32),
+             prefix_len=torch.zeros(G, dtype=torch.int32), group_off=torch.zeros(G + 1, dtype=torch.int32),
+             nq=nq, nkv=nkv, hd=hd, scale=1.0, out=torch.zeros(T, nq * hd), cu_q=None)
+    a.update(changed)
+    return {n: on_device(t) if isinstance(t, torch.Tensor) else t for n, t in a.items()}
+
+
+def test_a_consistent_call_launches_with_a_workspace_that_holds_all_parts(ops):
+    ops.shared_prefix_attention(**arguments())
+    (call,) = ops.calls
+    rows = 2 * 3 * 4 + 148 * 64
+    assert call[-4] == 32 * 3 + 16 + rows * (8 + 4 * 64) and call[-3] == 148 and ops.launches == 2
+
+
+@pytest.mark.parametrize("changed", [
+    dict(out=torch.zeros(3, 128)),
+    dict(out=torch.zeros(3, 256, dtype=torch.bfloat16)),
+    dict(qkv=torch.zeros(3, 255)),
+    dict(qkv=torch.zeros(3, 512)[:, ::2]),
+    dict(qkv=torch.zeros(3, 257)[:, :256]),                        # rows not on 16-byte boundaries
+    dict(qkv=torch.zeros(3 * 256 + 1)[1:].view(3, 256)),
+    dict(kcache=torch.zeros(9, 2, 16, 64).bfloat16()),
+    dict(vcache=torch.zeros(8, 2, 16, 64)),
+    dict(kcache=torch.zeros(9, 1, 16, 64), vcache=torch.zeros(9, 1, 16, 64)),
+    dict(kcache=torch.zeros(9, 2, 64, 16).transpose(2, 3)),
+    dict(block_table=torch.zeros(2, 5, dtype=torch.int32)),
+    dict(block_table=torch.zeros(3, 5, dtype=torch.int64)),
+    dict(ctx_len=torch.zeros(3)),
+    dict(group_off=torch.zeros(1, dtype=torch.int32)),
+    dict(cu_q=torch.zeros(3, dtype=torch.int32)),
+    dict(qkv=torch.zeros(4, 256), out=torch.zeros(4, 256)),        # one token per request, and four tokens
+    dict(hd=24, qkv=torch.zeros(3, 96), out=torch.zeros(3, 96), kcache=torch.zeros(9, 2, 16, 24), vcache=torch.zeros(9, 2, 16, 24)),
+    dict(nq=3, qkv=torch.zeros(3, 192), out=torch.zeros(3, 192)),
+])
+def test_refusals(ops, changed):
+    with pytest.raises(KernelError):
+        ops.shared_prefix_attention(**arguments(**changed))
+    assert not ops.calls and ops.launches == 0
+
+
+def test_a_tensor_of_the_host_or_another_device_is_refused(ops):
+    a = arguments()
+    a["ctx_len"] = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(KernelError):
+        ops.shared_prefix_attention(**a)
+    ops._device_index = 1
+    with pytest.raises(KernelError, match="device"):
+        ops.shared_prefix_attention(**arguments())
+    assert not ops.calls
+
+
+def test_what_the_launcher_refuses_is_an_error(ops):
+    ops._shared_attention = lambda *a: cuda.ERR_UNSUPPORTED
+    with pytest.raises(KernelError, match="not supported"):
+        ops.shared_prefix_attention(**arguments())
