@@ -116,6 +116,8 @@ class CudaOps:
         self._shared_attention = self.lib.somi_shared_attention
         p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
         self._shared_attention.argtypes = [p, i, n, p, p, p, i, p, p, p, p, i, i, i, i, i, i, i, i, ctypes.c_float, p, n, i, p, p]
+        self._draw = self.lib.somi_draw
+        self._draw.argtypes = [p, i, n, i, i, p, i, p, p, p, p, p, p, p, p, p, p]
         self.use_skinny_gemm = True
         self.skinny_max_tokens = int(self.lib.somi_skinny_gemm_max_tokens())
         self._retired: list = []
@@ -2194,6 +2196,59 @@ class CudaOps:
         self._done(rc, "sample")
         if trace.active():
             trace.note("sample", logits.numel() * 4)
+
+    def draw_tokens(self, logits, uniform, temperature, top_k, top_p, min_p, out, prob=None, penalty=None,
+                    hist_off=None, hist_tok=None) -> None:
+        """Tokens drawn from rows of logits with the caller's random numbers.
+
+        `logits` [rows, V] float32 or bfloat16 (rows may lie further apart); `uniform` float32 [rows] or
+        [rows, n], numbers in [0, 1): n draws of a row; `out` int32 and `prob` float32 (or None) of
+        the same shape: the tokens, and the probability that each was drawn with.  Per row: `temperature`
+        (<= 0: the lowest index of the maximum), `top_k` int32 (<= 0 or >= V: off), `top_p` (>= 1: off), `min_p` (<= 0: off).
+
+        Tokens are ordered by value, equal ones by index.  top-k keeps the first k; top-p keeps, of these, each in
+        front of which no more than top_p of their mass lies (the first always); min-p those with at
+        least min_p of the first one's probability.  The draw takes the first kept token in index order whose
+        cumulated mass is above uniform * (kept mass).  Probabilities below 2^-44 of the largest count
+        as 0; sums are exact sums of multiples of 2^-44, so equal rows give equal tokens whatever the
+        batch.  NaN logits count as -inf; a row without any other gives token 0 with probability 0.
+
+        `penalty` [rows] with `hist_off` int32 [rows + 1] and `hist_tok` int32 (a row's history, every token
+        once): repetition penalty in front of everything else (float32 logits), as in `sample`.
+        """
+        history = () if penalty is None else (penalty, hist_off, hist_tok)
+        if any(t is None for t in history):
+            raise KernelError("a repetition penalty comes with hist_off and hist_tok")
+        given = (uniform, temperature, top_k, top_p, min_p, out, *(() if prob is None else (prob,)), *history)
+        _check(*given)
+        if not (logits.is_cuda and logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
+            raise KernelError("logits are [rows, vocabulary] with contiguous rows on the device")
+        rows, V = logits.shape
+        if any(t.device != logits.device for t in given) or logits.device.index != self._device_index \
+                or torch.cuda.current_device() != self._device_index:
+            raise KernelError("draw_tokens: all tensors on the kernel table's device, which is the current one")
+        if uniform.dim() not in (1, 2) or uniform.shape[0] != rows or out.shape != uniform.shape \
+                or (prob is not None and prob.shape != uniform.shape) \
+                or any(t.numel() != rows for t in (temperature, top_k, top_p, min_p)) \
+                or (penalty is not None and (penalty.numel() != rows or hist_off.numel() != rows + 1)):
+            raise KernelError("draw_tokens takes uniform, out and prob of one shape, [rows] or [rows, draws], and settings [rows]")
+        if any(t.dtype != torch.float32 for t in (uniform, temperature, top_p, min_p, *(() if prob is None else (prob,)),
+                                                  *history[:1])) \
+                or any(t.dtype != torch.int32 for t in (top_k, out, *history[1:])):
+            raise KernelError("draw_tokens: float32 numbers and settings, int32 top_k, tokens and history")
+        if penalty is not None and logits.dtype != torch.float32:
+            raise KernelError("a repetition penalty takes float32 logits")
+        draws = uniform.shape[1] if uniform.dim() == 2 else 1
+        code = _code(logits)
+        if rows == 0 or draws == 0:
+            return
+        rc = self._draw(logits.data_ptr(), code, logits.stride(0), rows, V, uniform.data_ptr(), draws, temperature.data_ptr(),
+                        top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(), *(t.data_ptr() for t in history or ()),
+                        *(() if history else (None, None, None)), out.data_ptr(), None if prob is None else prob.data_ptr(),
+                        self._stream())
+        self._done(rc, "draw_tokens")
+        if trace.active():
+            trace.note("draw", rows * V * logits.element_size(), detail=f"{draws} draws" if draws > 1 else "")
 
     def uniform(self, seed: int, counter: int) -> float:
         """The uniform number in [0, 1) that row (seed, counter) draws (host evaluation)."""
