@@ -190,7 +190,8 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
         if (n.units <= 0) continue;
         const unsigned begin = n.begin + static_cast<unsigned>(kvh) * n.cost, end = begin + n.cost;
         // (what no request of a consistent call leads to)
-        if (n.cost != n.units + kOverhead || end > total || end < begin || n.place >= b.item_tokens) continue;
+        if (n.cost != n.units + kOverhead || end > total || end < begin ||
+            (n.place + 1) * b.per > block_rows) continue;
         for (unsigned cta = shares.cta_of(begin); cta < static_cast<unsigned>(ctas); ++cta) {
             const unsigned c0 = shares.begin(cta), c1 = shares.begin(cta + 1);
             if (c0 >= end) break;
@@ -198,9 +199,10 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
             if (o1 <= kOverhead || o1 <= o0) continue;              // it had only the item's fixed cost
             const size_t at = part_row(b, which == 0, o0 == 0, cta, block_rows, t, h, n.place * b.per + h % b.per);
             const float2 ml = parts.ml[at];
+            if (ml.x == -INFINITY && ml.y == 0.f) continue;         // none of its keys is seen
             const float now = fmaxf(m, ml.x);
-            if (now == -INFINITY) continue;          // none of its keys is seen
-            const float keep = exp2f(m - now), w = exp2f(ml.x - now);
+            const float ref = now == -INFINITY ? 0.f : now;         // (no number among its scores)
+            const float keep = exp2f(m - ref), w = exp2f(ml.x - ref);
             l = l * keep + ml.y * w;
             m = now;
 #pragma unroll
@@ -214,7 +216,7 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
             }
         }
     }
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
     for (int c = 0; c < COLS / 2; ++c) {
         const int col = (c * 32 + lane) * 4;
@@ -243,14 +245,18 @@ using namespace somi;
 using namespace somi::shp;
 
 // CTAs of a call (whichever kernel), and the rows of one CTA's continuation: what a caller needs for the workspace.
-static int shared_ctas(int hd, int per_sm) {
+static int shared_ctas(int per_sm) {
     int device = 0, sms = 0;
     cudaGetDevice(&device);
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) return 0;
     return sms * per_sm;
 }
-SOMI_API int somi_shared_attention_ctas(int hd) { return shared_ctas(hd, hd <= 64 ? 4 : hd <= 128 ? 2 : 1); }
-SOMI_API int somi_shared_attention_block_rows() { return kRows; }
+SOMI_API int somi_shared_attention_ctas(int hd, int tensor_cores) {
+    return shared_ctas(tensor_cores ? 1 : hd <= 64 ? 4 : hd <= 128 ? 2 : 1);
+}
+SOMI_API int somi_shared_attention_block_rows(int tensor_cores) {
+    return tensor_cores ? somi_shared_attention_tc_block_rows() : kRows;
+}
 
 // Bytes of workspace: notes, the header, maxima and sums, outputs.
 static long long workspace_bytes(long long T, int nq, int hd, int ctas, int block_rows) {
@@ -260,41 +266,45 @@ static long long workspace_bytes(long long T, int nq, int hd, int ctas, int bloc
 
 // qkv [T, >= nq hd] (rows `q_stride` elements apart), keys and values [num_pages, nkv, page_size, hd], block_table
 // [R, bt_stride], cu_q [R + 1] or null (then T = R, one token per request), ctx_len [R], group_off [G + 1], prefix_len [G];
-// `out` [T, nq hd].  Refuses what it cannot take; the lengths are read on the device.
+// `out` [T, nq hd].  `tensor_cores`: by attention_shared_tcgen05.cu (where somi_shared_attention_tc_takes says so).
+// Refuses what it cannot take; the lengths are read on the device.
 SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_stride, const void* keys, const void* values,
                                    const int* block_table, int bt_stride, const int* cu_q, const int* ctx_len,
                                    const int* prefix_len, const int* group_off, int T, int R, int G, int nq, int nkv, int hd,
-                                   int page_size, int num_pages, float scale, void* workspace, long long bytes, int ctas,
-                                   void* out, cudaStream_t stream) {
+                                   int page_size, int num_pages, float scale, int tensor_cores, void* workspace,
+                                   long long bytes, int ctas, void* out, cudaStream_t stream) {
     if (T <= 0 || R <= 0) return 0;
-    if (nkv <= 0 || nq <= 0 || nq % nkv || nq / nkv > kRows || hd % 16 || hd < 16 || hd > 256 || G < 0 || bt_stride <= 0 ||
+    if (nkv <= 0 || nq <= 0 || nq % nkv || (!tensor_cores && nq / nkv > kRows) || hd % 16 || hd < 16 || hd > 256 || G < 0 || bt_stride <= 0 ||
         page_size <= 0 || num_pages <= 0 || ctas <= 0 || static_cast<long long>(R) + G > kMaxEntries ||
         static_cast<long long>(R) + G > static_cast<long long>(ctas) * kOwned || (!cu_q && T != R))
         return SOMI_ERR_UNSUPPORTED;
     const long long span = static_cast<long long>(bt_stride) * page_size;
-    const int item_tokens = kRows / (nq / nkv);
+    if (tensor_cores && (dtype != SOMI_BF16 || !somi_shared_attention_tc_takes(nq, nkv, hd, page_size))) return SOMI_ERR_UNSUPPORTED;
+    const int block_rows = somi_shared_attention_block_rows(tensor_cores);
+    const int item_tokens = (tensor_cores ? block_rows / 2 : kRows) / (nq / nkv);
     const long long items = (R + static_cast<long long>(G) + 2 * (T / item_tokens + 1ll)) * nkv;
     if (span > 0x3fff0000ll || items * (span / kKeys + 3) > 0x7fffffffll || (static_cast<long long>(T) * nq + 7) / 8 > 0x7fffffffll)
         return SOMI_ERR_UNSUPPORTED;
-    if (bytes < workspace_bytes(T, nq, hd, ctas, kRows)) return SOMI_ERR_SCRATCH_TOO_SMALL;
+    if (bytes < workspace_bytes(T, nq, hd, ctas, block_rows)) return SOMI_ERR_SCRATCH_TOO_SMALL;
     Batch b{cu_q, ctx_len, prefix_len, group_off, block_table, bt_stride, R, G, T, nq, nkv, nq / nkv, page_size, num_pages,
             item_tokens, item_tokens, kKeys, kKeys, kKeys};
     char* at = static_cast<char*>(workspace);
     Note* notes = reinterpret_cast<Note*>(at);
     unsigned* header = reinterpret_cast<unsigned*>(at + 2ll * T * sizeof(Note));
-    const long long rows = 2ll * T * nq + static_cast<long long>(ctas) * kRows;
+    const long long rows = 2ll * T * nq + static_cast<long long>(ctas) * block_rows;
     Parts parts;
     parts.o = reinterpret_cast<float*>(header + 4);
     parts.ml = reinterpret_cast<float2*>(parts.o + rows * hd);
     const auto launch = [&](auto kind) {
         using E = decltype(kind);
-        int rc = hd <= 64    ? launch_shared<E, 64>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
-                 : hd <= 128 ? launch_shared<E, 128>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
-                             : launch_shared<E, 256>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream);
+        int rc = tensor_cores ? shared_attention_tc(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
+                 : hd <= 64   ? launch_shared<E, 64>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
+                 : hd <= 128  ? launch_shared<E, 128>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
+                              : launch_shared<E, 256>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream);
         if (rc) return rc;
         const long long out_rows = static_cast<long long>(T) * nq;
         return launch_pdl(shared_merge_kernel<E>, dim3(static_cast<unsigned>((out_rows + kMergeWarps - 1) / kMergeWarps)),
-                          dim3(kMergeWarps * 32), 0, stream, b, hd, notes, header, parts, ctas, kRows, static_cast<E*>(out));
+                          dim3(kMergeWarps * 32), 0, stream, b, hd, notes, header, parts, ctas, block_rows, static_cast<E*>(out));
     };
     return dtype == SOMI_F32 ? launch(float{}) : dtype == SOMI_BF16 ? launch(__nv_bfloat16{}) : SOMI_ERR_UNSUPPORTED;
 }

@@ -262,5 +262,12 @@ __device__ __forceinline__ size_t part_row(const Batch& b, bool prefix, bool fir
     return 2 * dense + static_cast<size_t>(cta) * block_rows + row_in_item;
 }
 
+// The tensor-core kernel (attention_shared_tcgen05.cu): sets its own sizes of tiles in `b`.
+int shared_attention_tc(Batch b, const void* q, long long q_stride, const void* keys, const void* values, int hd, float scale,
+                        Note* notes, unsigned* header, Parts parts, int ctas, cudaStream_t stream);
+
 }  // namespace shp
 }  // namespace somi
+
+SOMI_API int somi_shared_attention_tc_takes(int nq, int nkv, int hd, int page_size);
+SOMI_API int somi_shared_attention_tc_block_rows();

@@ -112,10 +112,12 @@ class CudaOps:
         self.lib.somi_decode_ring_chunks.restype = None
         self.use_tma_prefill = True
         self._gemm_maps: dict = {}
-        self._shared_plans: dict = {}      # (type, head size) -> CTAs and rows of a block of attention over shared prefixes
+        self.use_shared_tc = True
+        # type, heads, sizes -> whether on tensor cores, CTAs and rows of a block of attention over shared prefixes
+        self._shared_plans: dict = {}
         self._shared_attention = self.lib.somi_shared_attention
         p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-        self._shared_attention.argtypes = [p, i, n, p, p, p, i, p, p, p, p, i, i, i, i, i, i, i, i, ctypes.c_float, p, n, i, p, p]
+        self._shared_attention.argtypes = [p, i, n, p, p, p, i, p, p, p, p, i, i, i, i, i, i, i, i, ctypes.c_float, i, p, n, i, p, p]
         self._draw = self.lib.somi_draw
         self._draw.argtypes = [p, i, n, i, i, p, i, p, p, p, p, p, p, p, p, p, p]
         self.use_skinny_gemm = True
@@ -338,6 +340,9 @@ class CudaOps:
                               "its results are not valid")
         if int(self.lib.somi_gemm_f32_error()) != 0:
             raise KernelError("the float32 tcgen05 matrix product gave up waiting on a barrier; "
+                              "its results are not valid")
+        if int(self.lib.somi_shared_attention_error()) != 0:
+            raise KernelError("the tcgen05 attention over shared prefixes gave up waiting on a barrier; "
                               "its results are not valid")
         if int(self.lib.somi_chunks_error()) != 0:
             raise KernelError("the recurrence in chunks gave up waiting on a barrier; "
@@ -702,22 +707,25 @@ class CudaOps:
         if T == 0 or R == 0:
             return
         code = _code(qkv)
-        plan = self._shared_plans.get((code, hd))
+        key = (code, nq, nkv, hd, page_size, self.use_shared_tc)
+        plan = self._shared_plans.get(key)
         if plan is None:
-            plan = self._shared_plans[(code, hd)] = (int(self.lib.somi_shared_attention_ctas(ctypes.c_int(hd))),
-                                                     int(self.lib.somi_shared_attention_block_rows()))
-        ctas, block_rows = plan
+            tc = int(code == _BF16 and self.use_shared_tc
+                     and bool(self.lib.somi_shared_attention_tc_takes(nq, nkv, hd, page_size)))
+            plan = self._shared_plans[key] = (tc, int(self.lib.somi_shared_attention_ctas(hd, tc)),
+                                              int(self.lib.somi_shared_attention_block_rows(tc)))
+        tc, ctas, block_rows = plan
         rows = 2 * T * nq + ctas * block_rows
         work = torch.empty(32 * T + 16 + rows * (8 + 4 * hd), dtype=torch.uint8, device=qkv.device)
         rc = self._shared_attention(
             qkv.data_ptr(), code, qkv.stride(0), kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(),
             block_table.shape[1], None if cu_q is None else cu_q.data_ptr(), ctx_len.data_ptr(), prefix_len.data_ptr(),
-            group_off.data_ptr(), T, R, G, nq, nkv, hd, page_size, pages, scale, work.data_ptr(), work.numel(), ctas,
+            group_off.data_ptr(), T, R, G, nq, nkv, hd, page_size, pages, scale, tc, work.data_ptr(), work.numel(), ctas,
             out.data_ptr(), self._stream())
         self._done(rc, "shared_prefix_attention")
         self.launches += 1
         if trace.active():
-            trace.note("attention_shared", 2 * T * nq * hd * qkv.element_size(), detail="with merge; without keys and values")
+            trace.note("attention_shared_tcgen05" if tc else "attention_shared", 2 * T * nq * hd * qkv.element_size(), detail="with merge; without keys and values")
 
     def two_map_attention(self, qkv, kcache, vcache, batch, group, nq, nkv, d, vd, scale, window, keep,
                           factor: float, eps: float, gain: float, gate, out, storage=None) -> None:

@@ -78,6 +78,30 @@ def test_a_long_prefix_in_many_parts(ops, dtype):
     case.check(case.call(ops), sums(case))
 
 
+@pytest.mark.parametrize("nq,nkv,hd", [(28, 4, 128), (14, 2, 64), (4, 4, 128), (32, 1, 64)])
+def test_many_and_few_rows_in_turn(ops, nq, nkv, hd):
+    """Groups of more rows than a warp group holds beside groups of a few, portions of both kinds behind them: the two
+    ways of computing a piece follow each other many times in a call, and the rows of a group end anywhere in a tile."""
+    members = [[(i % 90, 1) for i in range(n)] for n in (40, 2, 75, 1, 19, 3, 150, 37)]
+    case = Case(nq, nkv, hd, 16, [(100 + 131 * g, m) for g, m in enumerate(members)], torch.bfloat16, seed=21,
+                loose=[(700, 1)] * 3)
+    case.check(case.call(ops), "bfloat16")
+    members = [[(i % 30, 1 + (7 * i) % t) for i in range(n)] for n, t in ((40, 2), (2, 90), (5, 40), (1, 300), (3, 1), (12, 33))]
+    case = Case(nq, nkv, hd, 16, [(700 - 131 * g, m) for g, m in enumerate(members)], torch.bfloat16, seed=22,
+                loose=[(0, 260), (5, 1), (0, 150)])
+    case.check(case.call(ops), "bfloat16")
+    ops.check_errors()
+
+
+def test_the_kernel_for_any_size_takes_what_the_tensor_cores_take(ops):
+    case = Case(14, 2, 64, 16, [(336, [(0, 5), (17, 1), (0, 131)])], torch.bfloat16, seed=23)
+    ops.use_shared_tc = False
+    try:
+        case.check(case.call(ops), "float32")
+    finally:
+        ops.use_shared_tc = True
+
+
 def test_far_apart_scores(ops):
     """The largest score lies in the prefix for one row and among its own keys for another, hundreds above the rest."""
     for dtype in (torch.bfloat16, torch.float32):

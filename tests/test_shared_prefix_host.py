@@ -18,10 +18,10 @@ def ops(monkeypatch):
     """A kernel table over CPU tensors whose launcher notes its calls."""
     table = cuda.CudaOps.__new__(cuda.CudaOps)
     table.launches, table._device_index, table.calls = 0, None, []
-    table._shared_plans = {}
+    table._shared_plans, table.use_shared_tc = {}, True
     table.lib = type("Library", (), {})()
-    table.lib.somi_shared_attention_ctas = lambda hd: 148
-    table.lib.somi_shared_attention_block_rows = lambda: 64
+    table.lib.somi_shared_attention_ctas = lambda hd, tc: 148
+    table.lib.somi_shared_attention_block_rows = lambda tc: 64
     table._shared_attention = lambda *a: table.calls.append(a) or 0
     table._stream = lambda: ctypes.c_void_p(0)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
