@@ -31,13 +31,15 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
 
     pdl_launch_dependents();
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const Range range = find_range<kThreads>(b, scratch);     // [descriptor]
+    __shared__ GroupScratch group_scratch;
+    const Groups groups = hold_groups(b, group_scratch);      // [descriptor]
+    const Range range = find_range<kThreads>(b, groups, scratch);
     pdl_wait();
-    write_notes<kThreads>(b, scratch, range.total, notes, header);
+    write_notes<kThreads>(b, groups, scratch, range.total, notes, header);
 
-    Walk walk(b, range);
+    Walk walk(b, groups, range);
     Piece p;
-    while (walk.next(b, p)) {
+    while (walk.next(b, groups, p)) {
         const int rows = p.tokens * b.per;
         __syncthreads();
         for (int i = tid; i < kRows * (HD / 4); i += kThreads) {
@@ -160,9 +162,10 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
     }
 }
 
-constexpr int kMergeWarps = 8;
+constexpr int kMergeWarps = 4;
 
-// A warp per (token, head).
+// A warp per (token, head).  A lane finds out where a part lies and loads its maximum and sum, for up to 32 parts at once;
+// then all lanes add the parts' outputs up, several loads in flight.
 template <typename T>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const unsigned* __restrict__ header, Parts parts,
@@ -173,52 +176,84 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
     const long long row = static_cast<long long>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
     if (row >= static_cast<long long>(b.T) * b.nq) return;
     const int t = static_cast<int>(row / b.nq), h = static_cast<int>(row % b.nq), kvh = h / b.per;
-    if (b.cu_q && (t < b.cu_q[0] || t >= b.cu_q[b.R])) return;     // a row of no request stays as it was
     const unsigned total = header[0];
+    const Note note[2] = {notes[t], notes[b.T + t]};                 // prefix, own keys (the first may be unwritten)
+    if (b.cu_q && (t < b.cu_q[0] || t >= b.cu_q[b.R])) return;       // a row of no request stays as it was
     if (total == 0) return;
     const Shares shares(total, ctas);
-    constexpr int COLS = 4;                          // of four columns a lane reads at a time: head sizes to 512
+    // the CTAs that had a part of the item, neighbours all
+    unsigned begin[2], first_cta[2], n_cta[2];
+    int place[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const Note& n = note[w];
+        place[w] = n.place & ((1 << 30) - 1);
+        begin[w] = n.begin + static_cast<unsigned>(kvh) * n.cost;
+        const unsigned end = begin[w] + n.cost;
+        // (the second half: what no note of a request's token looks like)
+        const bool there = (w == 1 || (note[1].place >> 30 & 1)) && n.units > 0 && n.cost == n.units + kOverhead && end <= total &&
+                           end >= begin[w] && place[w] >= 0 && (place[w] + 1) * b.per <= block_rows;
+        first_cta[w] = there ? shares.cta_of(begin[w]) : 0;
+        n_cta[w] = there ? shares.cta_of(end - 1) - first_cta[w] + 1 : 0;
+    }
+    const unsigned all = n_cta[0] + n_cta[1];
+    constexpr int COLS = 2;                          // of four columns a lane: head sizes to 256
     float m = -INFINITY, l = 0.f;
-    F4 o[COLS / 2];
+    F4 o[COLS];
 #pragma unroll
-    for (int c = 0; c < COLS / 2; ++c) o[c] = F4{{0.f, 0.f, 0.f, 0.f}};
-    const Note own = notes[b.T + t];
-    for (int which = 0; which < 2; ++which) {        // the prefix, then the request's own keys
-        if (which == 0 && !(own.place >> 30 & 1)) continue;
-        Note n = which == 0 ? notes[t] : own;
-        n.place &= (1 << 30) - 1;
-        if (n.units <= 0) continue;
-        const unsigned begin = n.begin + static_cast<unsigned>(kvh) * n.cost, end = begin + n.cost;
-        // (what no request of a consistent call leads to)
-        if (n.cost != n.units + kOverhead || end > total || end < begin ||
-            (n.place + 1) * b.per > block_rows) continue;
-        for (unsigned cta = shares.cta_of(begin); cta < static_cast<unsigned>(ctas); ++cta) {
-            const unsigned c0 = shares.begin(cta), c1 = shares.begin(cta + 1);
-            if (c0 >= end) break;
-            const unsigned o0 = c0 > begin ? c0 - begin : 0, o1 = min(c1, end) - begin;
-            if (o1 <= kOverhead || o1 <= o0) continue;              // it had only the item's fixed cost
-            const size_t at = part_row(b, which == 0, o0 == 0, cta, block_rows, t, h, n.place * b.per + h % b.per);
-            const float2 ml = parts.ml[at];
-            if (ml.x == -INFINITY && ml.y == 0.f) continue;         // none of its keys is seen
-            const float now = fmaxf(m, ml.x);
-            const float ref = now == -INFINITY ? 0.f : now;         // (no number among its scores)
-            const float keep = exp2f(m - ref), w = exp2f(ml.x - ref);
-            l = l * keep + ml.y * w;
-            m = now;
-#pragma unroll
-            for (int c = 0; c < COLS / 2; ++c) {
-                const int col = (c * 32 + lane) * 4;
-                if (col < d) {
-                    const F4 v = load4(parts.o + at * d + col);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[c].v[e] = fmaf(v.v[e], w, o[c].v[e] * keep);
-                }
+    for (int c = 0; c < COLS; ++c) o[c] = F4{{0.f, 0.f, 0.f, 0.f}};
+    for (unsigned p0 = 0; p0 < all; p0 += 32) {
+        const unsigned p = p0 + lane;
+        size_t at = 0;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (p < all) {
+            const int w = p < n_cta[0] ? 0 : 1;
+            const unsigned cta = first_cta[w] + (w ? p - n_cta[0] : p), c0 = shares.begin(cta), c1 = shares.begin(cta + 1);
+            const unsigned o0 = c0 > begin[w] ? c0 - begin[w] : 0, o1 = min(c1 - begin[w], static_cast<unsigned>(note[w].cost));
+            if (o1 > static_cast<unsigned>(kOverhead) && o1 > o0) {  // (else it had only the item's fixed cost)
+                at = part_row(b, w == 0, o0 == 0, cta, block_rows, t, h, place[w] * b.per + h % b.per);
+                ml = parts.ml[at];
             }
+        }
+        const bool some = !(ml.x == -INFINITY && ml.y == 0.f);      // (a part whose keys are all hidden has no output)
+        const float now = fmaxf(m, warp_max(ml.x)), ref = now == -INFINITY ? 0.f : now;
+        const float keep = exp2f(m - ref), weight = some ? exp2f(ml.x - ref) : 0.f;
+        l = l * keep + warp_sum(some ? ml.y * weight : 0.f);
+        m = now;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c].v[e] *= keep;
+        const unsigned live = __ballot_sync(0xffffffffu, some);
+        for (unsigned left = live; left != 0;) {
+            // up to four parts at a time
+            F4 v[4][COLS];
+            float w[4];
+            unsigned rest = left;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int from = rest ? __ffs(rest) - 1 : 0;
+                const size_t where = __shfl_sync(0xffffffffu, static_cast<unsigned long long>(at), from);
+                w[k] = __shfl_sync(0xffffffffu, weight, from);
+#pragma unroll
+                for (int c = 0; c < COLS; ++c)
+                    if (rest && (c * 32 + lane) * 4 < d) v[k][c] = load4(parts.o + where * d + (c * 32 + lane) * 4);
+                    else v[k][c] = F4{{0.f, 0.f, 0.f, 0.f}};
+                if (!rest) w[k] = 0.f;
+                rest &= rest - 1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[c].v[e] = fmaf(v[k][c].v[e], w[k], o[c].v[e]);
+            left = rest;
         }
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int c = 0; c < COLS / 2; ++c) {
+    for (int c = 0; c < COLS; ++c) {
         const int col = (c * 32 + lane) * 4;
         if (col < d) {
 #pragma unroll
@@ -261,7 +296,7 @@ SOMI_API int somi_shared_attention_block_rows(int tensor_cores) {
 // Bytes of workspace: notes, the header, maxima and sums, outputs.
 static long long workspace_bytes(long long T, int nq, int hd, int ctas, int block_rows) {
     const long long rows = 2 * T * nq + static_cast<long long>(ctas) * block_rows;
-    return 2 * T * static_cast<long long>(sizeof(Note)) + 16 + rows * 8 + rows * hd * 4;
+    return 2 * T * static_cast<long long>(sizeof(Note)) + 32 + rows * 8 + rows * hd * 4;
 }
 
 // qkv [T, >= nq hd] (rows `q_stride` elements apart), keys and values [num_pages, nkv, page_size, hd], block_table
@@ -283,8 +318,9 @@ SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_strid
     const int block_rows = somi_shared_attention_block_rows(tensor_cores);
     const int item_tokens = (tensor_cores ? block_rows / 2 : kRows) / (nq / nkv);
     const long long items = (R + static_cast<long long>(G) + 2 * (T / item_tokens + 1ll)) * nkv;
-    if (span > 0x3fff0000ll || items * (span / kKeys + 3) > 0x7fffffffll || (static_cast<long long>(T) * nq + 7) / 8 > 0x7fffffffll)
+    if (span > 0x3fff0000ll || items * (span / kKeys + 3) > 0x7fffffffll || static_cast<long long>(T) * nq / kMergeWarps >= 0x7fffffffll)
         return SOMI_ERR_UNSUPPORTED;
+    if (reinterpret_cast<uintptr_t>(workspace) % 32) return SOMI_ERR_UNSUPPORTED;
     if (bytes < workspace_bytes(T, nq, hd, ctas, block_rows)) return SOMI_ERR_SCRATCH_TOO_SMALL;
     Batch b{cu_q, ctx_len, prefix_len, group_off, block_table, bt_stride, R, G, T, nq, nkv, nq / nkv, page_size, num_pages,
             item_tokens, item_tokens, kKeys, kKeys, kKeys};
@@ -293,7 +329,7 @@ SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_strid
     unsigned* header = reinterpret_cast<unsigned*>(at + 2ll * T * sizeof(Note));
     const long long rows = 2ll * T * nq + static_cast<long long>(ctas) * block_rows;
     Parts parts;
-    parts.o = reinterpret_cast<float*>(header + 4);
+    parts.o = reinterpret_cast<float*>(header + 8);      // (on a boundary of 32 bytes, as the workspace is)
     parts.ml = reinterpret_cast<float2*>(parts.o + rows * hd);
     const auto launch = [&](auto kind) {
         using E = decltype(kind);

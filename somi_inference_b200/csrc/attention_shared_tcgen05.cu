@@ -42,6 +42,55 @@ constexpr int kMaxK = 4, kMaxV = 8;
 
 __device__ int g_shared_error = 0;
 
+// Eight floats at once, a whole sector of L2: a thread that writes a row by itself has no neighbours to fill it up.
+__device__ __forceinline__ void store8(float* to, const float* v) {
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(to), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+                 "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
+
+// 16 columns of the thread's row, arrived.  (The wait is in the same statement: between a load and its wait the registers
+// are the tensor memory's, and a compiler that copied or reused them there would not know.)
+__device__ __forceinline__ void ld16(uint32_t taddr, float* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
+          "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// All 128 columns, arrived.
+__device__ __forceinline__ void ld128(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+        "%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,"
+        "%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,%96,%97,%98,%99,%100,%101,%102,%103,%104,"
+        "%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,"
+        "%126,%127}, [%128];\n"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]),
+          "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]),
+          "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]),
+          "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]),
+          "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]), "=r"(r[81]),
+          "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]), "=r"(r[90]),
+          "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]),
+          "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]),
+          "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]),
+          "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]),
+          "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        : "r"(taddr)
+        : "memory");
+}
+
 struct PieceNote {
     int tiles;                                        // key tiles; < 0: no more pieces
     int key0, key_lo, key_hi;                         // first key of the first tile; keys there are
@@ -58,6 +107,7 @@ struct Tail {
     float2 b_state[kTile];                            // B's maximum and sum of each row, and A's maximum
     float a_top[kTile];
     PieceNote ring[kPieces];
+    GroupScratch groups;
     uint32_t tmem_base;
     int failed, softmax_failed[2];
 };
@@ -120,12 +170,13 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    const Range range = find_range<kTcThreads>(b, scratch);           // [descriptor]
+    const Groups groups = hold_groups(b, tail.groups);                // [descriptor]
+    const Range range = find_range<kTcThreads>(b, groups, scratch);   // [descriptor]
     t5::fence_before();
     __syncthreads();
     t5::fence_after();
     pdl_wait();
-    write_notes<kTcThreads>(b, scratch, range.total, notes, header);
+    write_notes<kTcThreads>(b, groups, scratch, range.total, notes, header);
     fence_proxy_async();                                              // (the scratch lies where copies will arrive)
     __syncthreads();
     const uint32_t tmem_s = tmem_base_s, tmem_o = tmem_base_s + 2 * kTile;
@@ -140,12 +191,12 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         if (warp == 11) {
             // ---- the pieces, one after the other
-            Walk walk(b, range);
+            Walk walk(b, groups, range);
             Piece p;
             int last_wide = -1;
             bool more = true, ok = true;
             for (int n = 0; more && ok; ++n) {
-                more = walk.next(b, p);
+                more = walk.next(b, groups, p);
                 ok = mbar_wait(smem_u32(&piece_empty[n % kPieces]), ((n / kPieces) & 1) ^ 1);
                 if (!ok) failed_s = 1;
                 if (lane == 0) {
@@ -241,7 +292,7 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                                       (static_cast<uint32_t>(kTile >> 4) << 24);
             const uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (static_cast<uint32_t>(HD >> 3) << 17) |
                                       (static_cast<uint32_t>(kTile >> 4) << 24);
-            const uint64_t q_desc[2] = {t5::desc_kmajor(smem_u32(Qs)), t5::desc_kmajor(smem_u32(Q1))};
+            const uint64_t q_desc = t5::desc_kmajor(smem_u32(Qs));
             const uint64_t k_desc = t5::desc_kmajor(smem_u32(Ks));
             const uint64_t v_desc = t5::desc_mnmajor(smem_u32(Vs), kHalf);
             bool ok = true;
@@ -257,77 +308,63 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                 }
                 t5::fence_after();
             };
-            int wide_at = 0, narrow_at[2] = {0, 0};                   // tiles of the pieces before
-            int done[2] = {0, 0};                                     // rounds of the warp groups before
+            int wide_at = 0, narrow_a = 0, narrow_b = 0;              // tiles of the pieces before
+            int done_a = 0, done_b = 0;                               // rounds of the warp groups before
             for (int n = 0; ok; ++n) {
                 wait(&piece_full[n % kPieces], (n / kPieces) & 1);
                 if (!ok) break;
                 const int nt = ring[n % kPieces].tiles, wide = ring[n % kPieces].wide;
                 if (nt < 0) break;
                 if (ring[n % kPieces].changed) t5::commit(smem_u32(&mode_done));
-                const int nx[2] = {wide ? nt : (nt + 1) / 2, wide ? (ring[n % kPieces].tokens > per_tile ? nt : 0) : nt / 2};
+                const int nx0 = wide ? nt : (nt + 1) / 2, nx1 = wide ? (ring[n % kPieces].tokens > per_tile ? nt : 0) : nt / 2;
                 mbar_arrive(smem_u32(&piece_empty[n % kPieces]));
-                auto k_stage = [&](int x, int i) { return wide ? (wide_at + i) % KST : x * KSN + (narrow_at[x] + i) % KSN; };
-                auto v_stage = [&](int x, int i) { return wide ? (wide_at + i) % VSW : x * VSN + (narrow_at[x] + i) % VSN; };
-                auto scores = [&](int x, int i) {                     // S_x = Q_x K^T
-                    const uint64_t kd = k_desc + ((k_stage(x, i) * TILE) >> 4);
-                    const uint64_t qd = wide ? q_desc[x] : q_desc[0];
-#pragma unroll
-                    for (int k16 = 0; k16 < HD / 16; ++k16)
-                        t5::mma_ss(tmem_s + x * kTile, qd + (((k16 >> 2) * kHalf + (k16 & 3) * 32) >> 4),
-                                   kd + (((k16 >> 2) * kHalf + (k16 & 3) * 32) >> 4), idesc_qk, k16 > 0 ? 1u : 0u);
-                    t5::commit(smem_u32(&s_full[x]));
-                };
-                auto outputs = [&](int x, int i) {                    // O_x += P_x V
-                    const uint64_t vd = v_desc + ((v_stage(x, i) * TILE) >> 4);
-#pragma unroll
-                    for (int k16 = 0; k16 < kTile / 16; ++k16)
-                        t5::mma_ts(tmem_o + x * kTile, tmem_s + x * kTile + 8 * k16, vd + ((k16 * 16 * 128) >> 4), idesc_pv,
-                                   (i > 0 || k16 > 0) ? 1u : 0u);
-                };
                 wait(&q_full, n & 1);
-                // the first tiles' arrival is tested here, the others' by the warp group that announces P
-                if (wide) {
-                    if (nt > 0) {
-                        wait(&k_full[1][k_stage(0, 0)], (wide_at / KST) & 1);
-                        if (ok) scores(0, 0);
-                        if (ok && nx[1]) scores(1, 0);
-                        if (ok) t5::commit(smem_u32(&k_empty[1][k_stage(0, 0)]));
-                    }
-                } else {
-                    for (int x = 0; x < 2; ++x)
-                        if (nx[x] > 0) {
-                            wait(&k_full[0][k_stage(x, 0)], (narrow_at[x] / KSN) & 1);
-                            if (!ok) break;
-                            scores(x, 0);
-                            t5::commit(smem_u32(&k_empty[0][k_stage(x, 0)]));
-                        }
-                }
-                for (int i = 0; i < nx[0] && ok; ++i) {
-#pragma unroll
+                // (one copy of each product in the code: this warp has few registers)
+                for (int i = -1; i < nx0 && ok; ++i) {
+#pragma unroll 1
                     for (int x = 0; x < 2; ++x) {
-                        if (i >= nx[x]) continue;
-                        spin(&p_full[x], (done[x] + i) & 1);
-                        if (!ok) break;
-                        outputs(x, i);
-                        if (i + 1 < nx[x]) scores(x, i + 1);
-                        if (!wide) {
-                            t5::commit(smem_u32(&v_empty[0][v_stage(x, i)]));
-                            if (i + 1 < nx[x]) t5::commit(smem_u32(&k_empty[0][k_stage(x, i + 1)]));
+                        const int n_x = x ? nx1 : nx0;
+                        if (i >= n_x) continue;
+                        const int k_at = (wide ? wide_at : x ? narrow_b : narrow_a) + i + 1;
+                        const int k_st = wide ? k_at % KST : x * KSN + k_at % KSN;
+                        const int v_st = wide ? (k_at - 1) % VSW : x * VSN + (k_at - 1) % VSN;
+                        if (i >= 0) {
+                            spin(&p_full[x], ((x ? done_b : done_a) + i) & 1);
+                            if (!ok) break;
+                            const uint64_t vd = v_desc + ((v_st * TILE) >> 4);          // O_x += P_x V
+#pragma unroll
+                            for (int k16 = 0; k16 < kTile / 16; ++k16)
+                                t5::mma_ts(tmem_o + x * kTile, tmem_s + x * kTile + 8 * k16, vd + ((k16 * 16 * 128) >> 4), idesc_pv,
+                                           (i > 0 || k16 > 0) ? 1u : 0u);
                         }
-                    }
-                    if (wide && ok) {
-                        t5::commit(smem_u32(&v_empty[1][v_stage(0, i)]));
-                        if (i + 1 < nt) t5::commit(smem_u32(&k_empty[1][k_stage(0, i + 1)]));
+                        if (i + 1 < n_x) {
+                            // the first tiles' arrival is tested here, the others' by the warp group that announces P
+                            if (i < 0 && (x == 0 || !wide)) wait(&k_full[wide][k_st], (wide ? k_at / KST : k_at / KSN) & 1);
+                            if (!ok) break;
+                            const uint64_t kd = k_desc + ((k_st * TILE) >> 4);          // S_x = Q_x K^T
+                            const uint64_t qd = q_desc + (wide && x ? (Q1 - Qs) >> 4 : 0);
+#pragma unroll
+                            for (int k16 = 0; k16 < HD / 16; ++k16)
+                                t5::mma_ss(tmem_s + x * kTile, qd + (((k16 >> 2) * kHalf + (k16 & 3) * 32) >> 4),
+                                           kd + (((k16 >> 2) * kHalf + (k16 & 3) * 32) >> 4), idesc_qk, k16 > 0 ? 1u : 0u);
+                            t5::commit(smem_u32(&s_full[x]));
+                        }
+                        if (!wide || x == (nx1 > 0)) {                                  // the tiles' last reader
+                            if (i >= 0) t5::commit(smem_u32(&v_empty[wide][v_st]));
+                            if (i + 1 < n_x) t5::commit(smem_u32(&k_empty[wide][k_st]));
+                        }
                     }
                 }
                 if (!ok) break;
                 t5::commit(smem_u32(&o_done));
-                for (int x = 0; x < 2; ++x) {
-                    done[x] += nx[x];
-                    if (!wide) narrow_at[x] += nx[x];
+                done_a += nx0;
+                done_b += nx1;
+                if (wide) {
+                    wide_at += nt;
+                } else {
+                    narrow_a += nx0;
+                    narrow_b += nx1;
                 }
-                if (wide) wide_at += nt;
             }
             if (!ok) failed_s = 1;                                    // the others run out of their bounded waits
         }
@@ -349,12 +386,14 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             constexpr int CH = HD / 8;                                // 16-byte pieces of a row
             constexpr int AT_ONCE = 32 / CH;                          // rows of one instruction
             const int chunk = lane % CH;
-            for (int r = r0 + lane / CH; p.tiles > 0 && r < r0 + rows_w; r += AT_ONCE) {
-                if (r >= live) break;
-                const int t = r / b.per;
-                const uint4 v = *reinterpret_cast<const uint4*>(
-                    q + (token0 + t) * q_stride + static_cast<size_t>(p.kvh * b.per + r - t * b.per) * HD + chunk * 8);
-                *reinterpret_cast<uint4*>(to + (chunk >> 3) * kHalf + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = v;
+            if (p.tiles > 0) {
+                for (int r = r0 + lane / CH; r < min(r0 + rows_w, live); r += AT_ONCE) {
+                    const int t = r / b.per;
+                    cp_async_16(smem_u32(to + (chunk >> 3) * kHalf + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)),
+                                q + (token0 + t) * q_stride + static_cast<size_t>(p.kvh * b.per + r - t * b.per) * HD + chunk * 8, 16);
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
             }
             fence_proxy_async();
             __syncwarp();
@@ -390,11 +429,16 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                 const int v_par = (wide ? v_at / VSW : v_at / VSN) & 1;
                 const bool edge = kb < lo || kb + kTile > p.key_hi;   // value rows that are none of the piece's
                 if (quarter == 0 || edge) ok = mbar_wait(smem_u32(vf), v_par, ok ? 400000 : 1) && ok;
-                if (quarter == 0 && i + 1 < n_x) {
+                // On behalf of the issuer: the next tile's keys, too, have arrived before P is announced.  A wait by parity
+                // wants to know that the stage's phase before has completed, so where a ring has one stage it comes
+                // behind this tile's scores (which were made of that phase's keys).
+                auto next_keys = [&]() {
                     const int k_at = v_at + 1;
                     const int k_st = wide ? k_at % KST : x * KSN + k_at % KSN;
                     ok = mbar_wait(smem_u32(&k_full[wide][k_st]), (wide ? k_at / KST : k_at / KSN) & 1, ok ? 400000 : 1) && ok;
-                }
+                };
+                const bool keys_late = KSN == 1 && !wide;
+                if (quarter == 0 && i + 1 < n_x && !keys_late) next_keys();
                 if (edge) {
                     const int pos = kb + row;
                     if (pos < lo || pos >= p.key_hi) {
@@ -408,13 +452,12 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                     fence_proxy_async();
                 }
                 ok = mbar_wait(smem_u32(&s_full[x]), (done + i) & 1, ok ? 400000 : 1) && ok;
+                __syncwarp();
                 t5::fence_after();
                 if (!idle) {
                     const bool inner = kb >= lo && kb + kTile <= first_end;       // every row sees all keys
                     uint32_t sv[128];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) t5::ld32_nowait(s_addr + c * 32, sv + c * 32);
-                    t5::wait_ld();
+                    ld128(s_addr, sv);
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (inner) {
 #pragma unroll
@@ -443,14 +486,15 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                     }
                     if (__any_sync(0xffffffffu, rescale)) {
                         // (the commit behind s_full covered the output products issued before)
+#pragma unroll 1
+                        for (int c = 0; c < HD / 16; ++c) {
+                            __syncwarp();
+                            float ov[16];
+                            uint32_t ow[16];
+                            ld16(o_addr + x * kTile + c * 16, ov);
 #pragma unroll
-                        for (int c = 0; c < HD / 32; ++c) {
-                            uint32_t ov[32];
-                            t5::ld32_nowait(o_addr + x * kTile + c * 32, ov);
-                            t5::wait_ld();
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
-                            t5::st32(o_addr + x * kTile + c * 32, ov);
+                            for (int j = 0; j < 16; ++j) ow[j] = __float_as_uint(ov[j] * alpha);
+                            t5::st16(o_addr + x * kTile + c * 16, ow);
                         }
                         t5::wait_st();
                         l *= alpha;
@@ -478,6 +522,7 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                     l += (s0 + s2) + (s1 + s3);
                     t5::wait_st();
                 }
+                if (quarter == 0 && i + 1 < n_x && keys_late) next_keys();
                 t5::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&p_full[x]));
@@ -486,6 +531,7 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             if (wide) wide_at += nt;
             else narrow_at += n_x;
             ok = mbar_wait(smem_u32(&o_done), n & 1, ok ? 400000 : 1) && ok;
+            __syncwarp();
             t5::fence_after();
             // the next piece's queries, so that its first scores are computed while this one's rows are written
             ok = get_piece(n + 1, ok);
@@ -498,17 +544,16 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             if (wide) {
                 if (mine) parts.ml[at] = make_float2(m, l);
                 if (n_x > 0 && !idle) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < HD / 32; ++c) {
-                        uint32_t v[32];
-                        t5::ld32_nowait(o_addr + x * kTile + c * 32, v);
-                        t5::wait_ld();
+                        // (the loads are the whole warp's: whatever a compiler makes of the condition below, it meets here)
+                        __syncwarp();
+                        float v[32];
+                        t5::ld32(o_addr + x * kTile + c * 32, v);
                         if (mine) {
-                            float4* to = reinterpret_cast<float4*>(parts.o + at * HD + c * 32);
+                            float* to = parts.o + at * HD + c * 32;
 #pragma unroll
-                            for (int d = 0; d < 32; d += 4)
-                                to[d / 4] = make_float4(__uint_as_float(v[d]), __uint_as_float(v[d + 1]), __uint_as_float(v[d + 2]),
-                                                        __uint_as_float(v[d + 3]));
+                            for (int d = 0; d < 32; d += 8) store8(to + d, v + d);
                         }
                     }
                 }
@@ -523,25 +568,23 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                 const float ca = a_top == -INFINITY ? 0.f : fast_exp2(a_top - top), cb = bs.x == -INFINITY ? 0.f : fast_exp2(bs.x - top);
                 if (mine && x == 0) parts.ml[at] = make_float2(top, l * ca + bs.y * cb);
                 if (nt > 0 && !idle) {
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        const uint32_t col = x * (HD / 2) + c * 16;
+                        __syncwarp();
+                        float y[16];
+                        ld16(o_addr + col, y);
 #pragma unroll
-                    for (int c = 0; c < HD / 64; ++c) {
-                        const uint32_t col = x * (HD / 2) + c * 32;
-                        uint32_t u[32], v[32];
-                        t5::ld32_nowait(o_addr + col, u);
-                        if (nt > 1) t5::ld32_nowait(o_addr + kTile + col, v);
-                        t5::wait_ld();
+                        for (int d = 0; d < 16; ++d) y[d] *= ca;
+                        if (nt > 1) {
+                            float v[16];
+                            ld16(o_addr + kTile + col, v);
+#pragma unroll
+                            for (int d = 0; d < 16; ++d) y[d] = fmaf(v[d], cb, y[d]);
+                        }
                         if (mine) {
-                            float4* to = reinterpret_cast<float4*>(parts.o + at * HD + col);
-#pragma unroll
-                            for (int d = 0; d < 32; d += 4) {
-                                float y[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    y[e] = __uint_as_float(u[d + e]) * ca;
-                                    if (nt > 1) y[e] = fmaf(__uint_as_float(v[d + e]), cb, y[e]);
-                                }
-                                to[d / 4] = make_float4(y[0], y[1], y[2], y[3]);
-                            }
+                            store8(parts.o + at * HD + col, y);
+                            store8(parts.o + at * HD + col + 8, y + 8);
                         }
                     }
                 }
@@ -557,6 +600,7 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     t5::fence_before();
     __syncthreads();
     if (warp == 9) {
+        __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base_s), "r"(TmemCols) : "memory");
     }
     if (tid == 0 && failed_s) atomicExch(&g_shared_error, 1);

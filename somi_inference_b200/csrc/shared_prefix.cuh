@@ -38,6 +38,11 @@ struct Batch {
     int unit_narrow, unit_wide, align;
 };
 
+// The groups' borders and prefixes as a block reads them: its own copies where they are few.
+struct Groups {
+    const int *off, *prefix;
+};
+
 // What joins the parts: per token, for the prefix and for its own keys, where the item of its first
 // key/value head begins in the order of costs, what an item costs, how many units it has, and the
 // token's place in the tile.
@@ -60,35 +65,35 @@ __device__ __forceinline__ int token_of(const Batch& b, int r) {
 }
 
 // The group that request r is in, or -1.  (Groups are runs of neighbouring requests.)
-__device__ __forceinline__ int group_of(const Batch& b, int r) {
+__device__ __forceinline__ int group_of(const Batch& b, const Groups& g, int r) {
     int lo = 0, hi = b.G;           // the last group that begins at or in front of r
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (ld_step(b.group_off + mid) <= r) lo = mid + 1;
+        if (g.off[mid] <= r) lo = mid + 1;
         else hi = mid;
     }
-    return lo > 0 && r < ld_step(b.group_off + lo) ? lo - 1 : -1;
+    return lo > 0 && r < g.off[lo] ? lo - 1 : -1;
 }
 
 // Everything that lengths lead to stays inside the batch's rows and the table's columns, whatever they hold.
-__device__ __forceinline__ Entry entry_of(const Batch& b, int e) {
+__device__ __forceinline__ Entry entry_of(const Batch& b, const Groups& gs, int e) {
     Entry x;
     const int span = b.bt_stride * b.page_size;
     if (e < b.G) {
-        const int r0 = clamped(ld_step(b.group_off + e), 0, b.R), r1 = clamped(ld_step(b.group_off + e + 1), r0, b.R);
+        const int r0 = clamped(gs.off[e], 0, b.R), r1 = clamped(gs.off[e + 1], r0, b.R);
         x.table = min(r0, b.R - 1);
         x.first = token_of(b, r0);
         x.tokens = r1 > r0 ? max(token_of(b, r1) - x.first, 0) : 0;
         x.key_lo = 0;
-        x.key_hi = clamped(ld_step(b.prefix_len + e), 0, min(span, max(0, ld_step(b.ctx_len + x.table))));
+        x.key_hi = clamped(gs.prefix[e], 0, min(span, max(0, ld_step(b.ctx_len + x.table))));
         x.pos0 = 0x3fffffff;        // every token sees the whole prefix
     } else {
-        const int r = e - b.G, g = group_of(b, r);
+        const int r = e - b.G, g = group_of(b, gs, r);
         x.table = r;
         x.first = token_of(b, r);
         x.tokens = b.cu_q ? max(token_of(b, r + 1) - x.first, 0) : 1;
         const int ctx = clamped(ld_step(b.ctx_len + r), 0, span);
-        x.key_lo = g >= 0 ? clamped(ld_step(b.prefix_len + g), 0, ctx) : 0;
+        x.key_lo = g >= 0 ? clamped(gs.prefix[g], 0, ctx) : 0;
         x.key_hi = min(ctx + x.tokens, span);
         x.pos0 = ctx;
     }
@@ -125,15 +130,30 @@ struct RangeScratch {
     unsigned owned[kOwned];
 };
 
+constexpr int kGroupsHeld = 31;     // groups that a block copies
+struct GroupScratch {
+    int off[kGroupsHeld + 1], prefix[kGroupsHeld + 1];
+};
+
+// All threads of the block, first of all.
+__device__ __forceinline__ Groups hold_groups(const Batch& b, GroupScratch& s) {
+    if (b.G > kGroupsHeld) return Groups{b.group_off, b.prefix_len};
+    const int i = threadIdx.x;
+    if (i <= b.G) s.off[i] = ld_step(b.group_off + i);
+    if (i >= 32 && i - 32 < b.G) s.prefix[i - 32] = ld_step(b.prefix_len + i - 32);
+    __syncthreads();
+    return Groups{s.off, s.prefix};
+}
+
 // All threads of the block.  Writes the notes of the entries that this CTA owns and header[0] = all costs (CTA 0).
 template <int THREADS>
-__device__ __forceinline__ Range find_range(const Batch& b, RangeScratch& s) {
+__device__ __forceinline__ Range find_range(const Batch& b, const Groups& gs, RangeScratch& s) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int E = b.G + b.R, each = (E + THREADS - 1) / THREADS;
     const int e0 = tid * each, e1 = min(e0 + each, E);
     unsigned mine = 0, first_cost = 0;
     for (int e = e0; e < e1; ++e) {
-        const Entry x = entry_of(b, e);
+        const Entry x = entry_of(b, gs, e);
         const unsigned c = static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
         if (e == e0) first_cost = c;
         mine += c;
@@ -164,7 +184,7 @@ __device__ __forceinline__ Range find_range(const Batch& b, RangeScratch& s) {
     for (int e = e0; e < e1; ++e) {
         unsigned c = first_cost;
         if (each > 1) {
-            const Entry x = entry_of(b, e);
+            const Entry x = entry_of(b, gs, e);
             c = static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
         }
         if (holds && r.begin >= at && r.begin < at + c) {
@@ -182,11 +202,11 @@ __device__ __forceinline__ Range find_range(const Batch& b, RangeScratch& s) {
 
 // The notes of this CTA's entries.  `notes`: [2][T], prefixes first.  After the wait for the kernels in front.
 template <int THREADS>
-__device__ __forceinline__ void write_notes(const Batch& b, const RangeScratch& s, unsigned total, Note* notes,
+__device__ __forceinline__ void write_notes(const Batch& b, const Groups& gs, const RangeScratch& s, unsigned total, Note* notes,
                                             unsigned* header) {
     if (blockIdx.x == 0 && threadIdx.x == 0) header[0] = total;
     for (int e = blockIdx.x, k = 0; e < b.G + b.R; e += gridDim.x, ++k) {
-        const Entry x = entry_of(b, e);
+        const Entry x = entry_of(b, gs, e);
         if (e < b.G && x.tiles == 0) continue;      // the requests' own notes say that there is no prefix
         Note* to = notes + (e < b.G ? 0 : b.T) + x.first;
         for (int t = threadIdx.x; t < x.tokens; t += THREADS) {
@@ -218,16 +238,16 @@ struct Walk {
     int e;
     unsigned base;
     Entry x;
-    __device__ __forceinline__ Walk(const Batch& b, const Range& r) : at(r.begin), end(r.end), e(r.entry), base(r.entry_base) {
-        if (at < end) x = entry_of(b, e);
+    __device__ __forceinline__ Walk(const Batch& b, const Groups& gs, const Range& r) : at(r.begin), end(r.end), e(r.entry), base(r.entry_base) {
+        if (at < end) x = entry_of(b, gs, e);
     }
-    __device__ __forceinline__ bool next(const Batch& b, Piece& p) {
+    __device__ __forceinline__ bool next(const Batch& b, const Groups& gs, Piece& p) {
         while (at < end) {
             unsigned whole = static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
             while (at >= base + whole) {            // (the range ends inside an entry, so this ends)
                 base += whole;
                 if (++e >= b.G + b.R) return false;
-                x = entry_of(b, e);
+                x = entry_of(b, gs, e);
                 whole = static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
             }
             const unsigned cost = x.cost();

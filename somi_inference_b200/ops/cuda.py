@@ -716,7 +716,7 @@ class CudaOps:
                                               int(self.lib.somi_shared_attention_block_rows(tc)))
         tc, ctas, block_rows = plan
         rows = 2 * T * nq + ctas * block_rows
-        work = torch.empty(32 * T + 16 + rows * (8 + 4 * hd), dtype=torch.uint8, device=qkv.device)
+        work = torch.empty(32 * T + 32 + rows * (8 + 4 * hd), dtype=torch.uint8, device=qkv.device)
         rc = self._shared_attention(
             qkv.data_ptr(), code, qkv.stride(0), kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(),
             block_table.shape[1], None if cu_q is None else cu_q.data_ptr(), ctx_len.data_ptr(), prefix_len.data_ptr(),

@@ -93,6 +93,21 @@ def test_many_and_few_rows_in_turn(ops, nq, nkv, hd):
     ops.check_errors()
 
 
+@pytest.mark.parametrize("nq,nkv,hd", [(28, 4, 128), (14, 2, 64)])
+def test_long_pieces_from_cold_memory(ops, nq, nkv, hd):
+    """Pieces of many key tiles whose maxima grow on the way (large scores), with keys and values that no cache holds:
+    a copy may arrive long after it was asked for."""
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    for members, prefix in ((40, 6000), (2, 9000), (9, 3000)):
+        case = Case(nq, nkv, hd, 16, [(prefix, [(17 * i % 90, 1) for i in range(members)])] * 2, torch.bfloat16, seed=members,
+                    loose=[(2500, 1)] * 40, scale=0.5)
+        for _ in range(3):
+            flush.fill_(1)
+            case.call(ops)
+        case.check(case.out, "bfloat16")
+    ops.check_errors()
+
+
 def test_the_kernel_for_any_size_takes_what_the_tensor_cores_take(ops):
     case = Case(14, 2, 64, 16, [(336, [(0, 5), (17, 1), (0, 131)])], torch.bfloat16, seed=23)
     ops.use_shared_tc = False

@@ -42,7 +42,7 @@ def test_a_consistent_call_launches_with_a_workspace_that_holds_all_parts(ops):
     ops.shared_prefix_attention(**arguments())
     (call,) = ops.calls
     rows = 2 * 3 * 4 + 148 * 64
-    assert call[-4] == 32 * 3 + 16 + rows * (8 + 4 * 64) and call[-3] == 148 and ops.launches == 2
+    assert call[-4] == 32 * 3 + 32 + rows * (8 + 4 * 64) and call[-3] == 148 and ops.launches == 2
 
 
 @pytest.mark.parametrize("changed", [
