@@ -7,21 +7,29 @@
 //     draw: the first i in index order whose cumulated mass over kept tokens is above u (kept mass)
 //
 // Which token a number falls on, and where a cut lies, is a comparison of sums, so these must not depend
-// on the order of summation nor on float32's rounding: a weight is computed in float64 (2^r by its Taylor
-// polynomial, |r| <= 1/2, relative error 2e-16) and held as an integer multiple of 2^-44, and sums of integers
-// are exact.  (Fewer than 2^20 weights of at most 2^44 stay below 2^64.)  So the result is the same bits
+// on the order of summation nor on float32's rounding: a weight is computed to 2^-37 of itself (`Heat::weight`)
+// and held as an integer multiple of 2^-44, and sums of integers are exact.  (Fewer than 2^20 weights of at most 2^44 stay below 2^64.)  So the result is the same bits
 // whatever the launch looks like, and differs from real arithmetic only where a border lies within
 // about 1e-11 of the number.
 //
-// A cluster of CTAs shares a row; each holds its slice in shared memory, read from HBM once.  A warp owns a
-// contiguous segment of it.  All three cuts keep a beginning of one order, so what is kept is a key (the
-// order-preserving integer image of a float), and an index up to which logits equal to it are kept.  The key
-// is found by histograms that the cluster's CTAs add up: first over the logits' distance from
-// the maximum (1,024 bins over the 30.5 temperatures in which weights do not vanish, so that a bin holds few
-// tokens), then over the keys that lie in the bin of the cut, until a bin is one key.
+// A cluster of CTAs shares a row; each holds its slice in shared memory, read from HBM once, as a bulk copy where
+// the row is aligned.  A warp owns a contiguous segment of it.  All three cuts keep a beginning of one order, so a
+// token can be left out as soon as it is known to lie behind a cut:
+//     top-k: the r-th largest of a CTA's warps' (or threads') maxima, r = k / (CTAs of the cluster), has r logits at or above
+//            it in that CTA, so the least such value of the cluster has k at or above it in the row;
+//     top-p: the masses of 1,024 bins of the logits' distance from the maximum say in which bin the cut lies;
+//     min-p: by its definition.
+// What is left (the survivors, in the order of their indices) is usually a few dozen to a few hundred tokens; they are collected in one
+// CTA, sorted, cut and drawn from there: a row of 152,064 logits costs a pass for its maximum and one that
+// looks for survivors, and only a row with top-p and without top-k a weight for every token.  Where more than
+// `kListed` survive, the cuts are found by histograms that the cluster's CTAs add up: first those bins (they
+// span the 30.5 temperatures in which weights do not vanish), then the keys (the order-preserving integer image of a
+// float) that lie in the bin of the cut, until a bin is one key; what is kept is then a key and an index up to which logits equal to it are
+// kept, and weights are computed a second time to find where the numbers fall.
 #include <cooperative_groups.h>
 
-#include "common.cuh"
+#include "tma.cuh"
+#include "mma.cuh"
 
 namespace somi {
 namespace draw {
@@ -29,7 +37,10 @@ namespace draw {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kMaxCluster = 16;
+constexpr int kMassBins = 2048;              // of the masses that top-p cuts
+constexpr int kListed = 1024;                // survivors that one CTA takes
 constexpr int kFraction = 44;                // a weight is an integer multiple of 2^-44
+constexpr int kCopies = 16;                  // of the table of powers
 typedef unsigned long long u64;
 
 struct Settings {
@@ -37,18 +48,41 @@ struct Settings {
     const int *top_k, *hist_off, *hist_tok;
 };
 
+struct Token { unsigned key; int at; };
+
 struct Shared {
-    u64 hist[2][kBins];                      // (read by the other CTAs of the cluster)
+    union {
+        struct {
+            union {
+                u64 hist[2][kBins];          // (read by the other CTAs of the cluster)
+                struct {
+                    Token list[kListed];     // this CTA's survivors (read by the first CTA)
+                    Token bin_list[kListed]; // its tokens of the cut's bin (likewise)
+                };
+                struct {
+                    u64 order[kListed];      // in the first CTA: all of them by value,
+                    u64 weight[kListed];     // and their weights
+                };
+            };
+            Token all[kListed];              // the first CTA: the row's survivors
+        };
+        unsigned pieces[3][kMassBins];       // masses of bins in pieces of 15 bits (read by the other CTAs)
+    };
+    u64 powers[64 * kCopies];
     u64 scan[kWarps];
     u64 warp_sum[kWarps];
     u64 total[kMaxCluster], mass[kMaxCluster];   // written by the other CTAs, one exchange each
-    unsigned top_key[kMaxCluster], top_at[kMaxCluster], ties[kMaxCluster];
+    unsigned top_key[kMaxCluster], floor_key[kMaxCluster], top_at[kMaxCluster], ties[kMaxCluster];
+    uint2 listed[kMaxCluster];               // survivors, tokens of the cut's bin
     unsigned key[kWarps], at[kWarps];
     u64 cross_above, cross_mass;
-    int cross_bin;
+    int cross_bin, tie_cut;
+    unsigned cut_key;
     unsigned lo, hi;
-    int tie_cut;
+    unsigned long long loaded;               // mbarrier of the bulk copy
 };
+
+__device__ int g_draw_error = 0;
 
 __device__ __forceinline__ unsigned key_of(float x) {
     const unsigned u = __float_as_uint(x);
@@ -60,7 +94,7 @@ __device__ __forceinline__ float value_of(unsigned key) {
 // A logit: NaN counts as -inf, -0 as 0 (equal values must have equal keys).
 __device__ __forceinline__ float logit_of(float x) { return x == x ? x + 0.0f : -INFINITY; }
 
-// 2^r = 1 + r ln 2 (1 + r ln 2 / 2 (1 + r ln 2 / 3 (...))), to the N-th power of r
+// 2^r = 1 + r ln 2 (1 + r ln 2 / 2 (1 + r ln 2 / 3 (...))), to the N-th power of r (|r| <= 1/2, N = 13: 2e-16)
 template <int N, int K = 0>
 __device__ __forceinline__ double exp2_taylor(double r) {
     if constexpr (K == N) return 1.0;
@@ -71,7 +105,10 @@ __device__ __forceinline__ double exp2_taylor(double r) {
 struct Heat {
     float top;
     double c;                                // log2(e) / T
-    float bins;                              // bins per unit of distance from the maximum
+    float bins;                              // 1 / the distance from the maximum at which bins end
+    float low;                               // below it every weight is nothing
+    const u64* powers;                       // 2^(62 + j / 64) at kCopies j, j = 0 .. 63: this lane's copy
+    bool plain;                              // the maximum is not so large that its neighbours have no weight
 
     // w 2^44 before it is rounded to an integer; 0 where w < 2^-44
     __device__ __forceinline__ double scaled(float x) const {
@@ -85,13 +122,30 @@ struct Heat {
         const double p = exp2_taylor<13>(r);
         return __longlong_as_double(__double_as_longlong(p) + (static_cast<long long>(n + kFraction) << 52));
     }
+    // The integer.  float64 operations are rare here (16 a cycle and SM): three of them make y = (x - max) c + 1536, whose
+    // low 42 bits are the fraction of y, the next ten 512 + its floor; 2^fraction is a table's value for six bits times
+    // 1 + r a1 + .. + r^4 a4, r below 2^-6 and held to 2^-38, in 32-bit integers (a_k = ln(2)^k / k!).  Relative error at
+    // most 2^-37.  The table has a copy for every two lanes of a warp, since lanes that read different entries of one copy
+    // meet in the same banks.
     __device__ __forceinline__ u64 weight(float x) const {
-        const double shifted = scaled(x) + 4503599627370496.0;         // 2^52: the integer is in the low bits
-        return static_cast<u64>(__double_as_longlong(shifted)) & ((1ull << 52) - 1);
+        if (!plain) return static_cast<u64>(__double_as_longlong(scaled(logit_of(x)) + 4503599627370496.0)) & ((1ull << 52) - 1);
+        const double d = static_cast<double>(fmaxf(x, low)) - static_cast<double>(top);
+        const double v = fma(d, c, 1536.0);
+        const unsigned hi = static_cast<unsigned>(__double2hiint(v));
+        const unsigned r = __funnelshift_r(static_cast<unsigned>(__double2loint(v)), hi, 4);
+        const int n = 512 - static_cast<int>((hi >> 10) & 1023u);      // -floor(y)
+        const u64 t = powers[((hi >> 4) & 63u) * kCopies];
+        unsigned e = 58200u + __umulhi(r, 158u);                       // a3 2^20, a4 2^14
+        e = 16121328u + __umulhi(r, e);                                // a2 2^26
+        e = 2977044472u + __umulhi(r, e);                              // a1 2^32
+        e = __umulhi(r, e);                                            // (2^(r / 2^38) - 1) 2^38
+        const u64 whole = t + ((static_cast<u64>(static_cast<unsigned>(t >> 32)) * e) >> 6);
+        return n > kFraction ? 0ull : (whole + (1ull << (61 - kFraction + n))) >> (62 - kFraction + n);
     }
     // falls (or stays) as x grows
+    template <int BINS>
     __device__ __forceinline__ int bin(float x) const {
-        return x == top ? 0 : static_cast<int>(fminf((top - x) * bins, static_cast<float>(kBins - 1)));
+        return x == top ? 0 : static_cast<int>(fminf((top - x) * (bins * (BINS - 1)), static_cast<float>(BINS - 1)));
     }
 };
 
@@ -130,21 +184,28 @@ __device__ __forceinline__ unsigned first_key(unsigned lo, unsigned hi, int lane
     return lo;
 }
 
+// The keys of logits in [klo, khi] that fall into bin `bin` (counted from the maximum).  One warp.
+template <int BINS>
+__device__ __forceinline__ void keys_of_bin(const Heat& heat, int bin, int lane, unsigned& klo, unsigned& khi) {
+    const unsigned lo = first_key(klo, khi, lane, [&](unsigned k) { return heat.template bin<BINS>(value_of(k)) <= bin; });
+    if (bin > 0) khi = first_key(lo, khi, lane, [&](unsigned k) { return heat.template bin<BINS>(value_of(k)) < bin; }) - 1;
+    klo = lo;
+}
+
 // The cut of an order at `target`: the last key of which some token has (mass of larger keys) <= target.
 struct Cut {
     unsigned key;
     u64 above, mass;                         // of larger keys; of the logits equal to it
 };
 
-// MASS: weights; else every token counts 1.  Tokens with keys below `floor_key` are left out.
+// MASS: weights; else every token counts 1.  The cut lies in keys [klo, khi]; `above` is the mass of larger ones; `binned`: they
+// are one bin of the first histogram.
 template <bool MASS, typename At>
-__device__ Cut find_cut(cg::cluster_group& cluster, Shared& s, const Heat& heat, At at, int lo_i, int hi_i, unsigned floor_key,
-                        u64 target, int& level) {
+__device__ Cut find_cut(cg::cluster_group& cluster, Shared& s, const Heat& heat, At at, int lo_i, int hi_i, unsigned klo,
+                        unsigned khi, u64 above, bool binned, u64 target, int& level) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned ranks = cluster.num_blocks();
-    unsigned klo = floor_key, khi = key_of(heat.top);
-    u64 above = 0;
-    for (int pass = 0;; ++pass, ++level) {
+    for (int pass = binned ? 1 : 0;; ++pass, ++level) {
         u64* hist = s.hist[level & 1];
         for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
         if (tid == 0) s.cross_bin = kBins;
@@ -155,7 +216,7 @@ __device__ Cut find_cut(cg::cluster_group& cluster, Shared& s, const Heat& heat,
             const float x = at(i);
             const unsigned key = key_of(x);
             if (key < klo || key > khi) continue;
-            const int bin = pass == 0 ? kBins - 1 - heat.bin(x) : static_cast<int>((key - klo) >> shift);
+            const int bin = pass == 0 ? kBins - 1 - heat.bin<kBins>(x) : static_cast<int>((key - klo) >> shift);
             const u64 w = MASS ? heat.weight(x) : 1ull;
             if (w) atomicAdd(hist + bin, w);
         }
@@ -187,9 +248,8 @@ __device__ Cut find_cut(cg::cluster_group& cluster, Shared& s, const Heat& heat,
             }
         if (pass == 0 && warp == 0) {
             // the keys whose logits fall into the bin
-            const int bin = kBins - 1 - cross;
-            const unsigned lo = first_key(klo, khi, lane, [&](unsigned k) { return heat.bin(value_of(k)) <= bin; });
-            const unsigned hi = bin == 0 ? khi : first_key(lo, khi, lane, [&](unsigned k) { return heat.bin(value_of(k)) < bin; }) - 1;
+            unsigned lo = klo, hi = khi;
+            keys_of_bin<kBins>(heat, kBins - 1 - cross, lane, lo, hi);
             if (lane == 0) {
                 s.lo = lo;
                 s.hi = hi;
@@ -214,12 +274,86 @@ __device__ Cut find_cut(cg::cluster_group& cluster, Shared& s, const Heat& heat,
     }
 }
 
+// f(index, logit) for a warp's segment [lo_i, hi_i), 16 bytes of logits a lane at a time (not in the order of indices).
+template <typename T, typename F>
+__device__ __forceinline__ void each_logit(const T* seg, int n, int lane, F f) {
+    constexpr int VEC = 16 / sizeof(T);
+    const int whole = n / VEC;
+    for (int i = lane; i < whole; i += 32) {
+        const uint4 q = reinterpret_cast<const uint4*>(seg)[i];
+        const T* v = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f(i * VEC + e, to_float(v[e]));
+    }
+    for (int i = whole * VEC + lane; i < n; i += 32) f(i, to_float(seg[i]));
+}
+
+// Inclusive scan over the block, in the order of threads.  Ends with all threads together.
+__device__ __forceinline__ u64 block_scan64(u64 v, u64* scratch, u64& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u64 incl = warp_scan64(v, lane);
+    __syncthreads();
+    if (lane == 31) scratch[warp] = incl;
+    __syncthreads();
+    u64 before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const u64 x = scratch[w];
+        if (w < warp) before += x;
+        sum += x;
+    }
+    total = sum;
+    return before + incl;
+}
+
+// `n` different numbers of v in descending order, by their ranks or, where they are many, in a network.  Zeros behind them up to a
+// power of two.  Begins and ends with all threads together.
+__device__ __forceinline__ void sort_descending(u64* v, int n) {
+    const int tid = threadIdx.x;
+    if (n <= kThreads / 2) {
+        // 512 / size threads a number, neighbours in a warp (at most 32)
+        int size = 16;
+        while (size < n) size *= 2;
+        const int each = kThreads / size, i = tid / each, part = tid % each;
+        const u64 mine = i < n ? v[i] : 0ull;
+        unsigned rank = 0;
+        if (i < n)
+            for (int j = part; j < n; j += each) rank += v[j] > mine ? 1u : 0u;
+        for (int o = 1; o < each; o *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        __syncthreads();
+        if (i < n && part == 0) v[rank] = mine;
+        __syncthreads();
+        return;
+    }
+    int size = kThreads;
+    while (size < n) size *= 2;
+    for (int i = n + tid; i < size; i += kThreads) v[i] = 0ull;
+    for (int run = 2; run <= size; run *= 2)
+        for (int step = run / 2; step > 0; step /= 2) {
+            __syncthreads();
+            for (int t = tid; t < size / 2; t += kThreads) {
+                const int i = 2 * t - (t & (step - 1)), j = i + step;
+                const u64 a = v[i], b = v[j];
+                if ((a < b) == ((i & run) == 0)) {
+                    v[i] = b;
+                    v[j] = a;
+                }
+            }
+        }
+    __syncthreads();
+}
+
+__device__ __forceinline__ u64 drawn_mass(float u, u64 z) {
+    const u64 target = u > 0.f ? static_cast<u64>(static_cast<double>(u) * static_cast<double>(z)) : 0ull;
+    return min(target, z - 1);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Settings set, const float* __restrict__ uniform,
             int draws, int* __restrict__ out, float* __restrict__ prob) {
     extern __shared__ __align__(16) unsigned char slice_raw[];
-    __shared__ Shared s;
+    __shared__ __align__(16) Shared s;
     T* slice = reinterpret_cast<T*>(slice_raw);                // kWarps segments of `seg`
     cg::cluster_group cluster = cg::this_cluster();
     const unsigned rank = cluster.block_rank(), ranks = cluster.num_blocks();
@@ -227,117 +361,434 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = (static_cast<int>(rank) * kWarps) * seg;       // the CTA's first token
     const int lo_i = min(first + warp * seg, V), hi_i = min(first + (warp + 1) * seg, V);
+    const int mine_n = hi_i - lo_i;                            // logits of this warp's segment
 
     pdl_launch_dependents();
+    if (tid == 0) {
+        mbar_init(smem_u32(&s.loaded), 1);
+        mbar_fence_init();
+    }
     pdl_wait();
-    const T* x_row = logits + row * stride;
-    for (int i = lo_i + lane; i < hi_i; i += 32) slice[i - first] = x_row[i];
+    const T* x_row = logits + row * stride + first;
+    const int slice_n = max(min(first + kWarps * seg, V) - first, 0);
+    const bool bulk = (reinterpret_cast<uintptr_t>(x_row) & 15) == 0;
+    const int bulk_n = bulk ? slice_n / (16 / static_cast<int>(sizeof(T))) * (16 / static_cast<int>(sizeof(T))) : 0;
+    __syncthreads();
+    if (tid == 0 && bulk_n > 0) {
+        const uint32_t bytes = static_cast<uint32_t>(bulk_n) * sizeof(T);
+        mbar_expect_tx(smem_u32(&s.loaded), bytes);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(slice)),
+                     "l"(x_row), "r"(bytes), "r"(smem_u32(&s.loaded))
+                     : "memory");
+    }
+    for (int i = bulk_n + tid; i < slice_n; i += kThreads) slice[i] = x_row[i];
+    // (while the logits are on their way)
+    for (int i = tid; i < 64 * kCopies; i += kThreads) {
+        const int j = i / kCopies;
+        const double t = exp2_taylor<13>((j < 32 ? j : j - 64) * (1.0 / 64.0)) * (j < 32 ? 4611686018427387904.0 : 9223372036854775808.0);
+        s.powers[i] = static_cast<u64>(t);
+    }
     const float heat_in = set.temperature[row];
+    const int k_in = set.top_k[row];
+    const float p = set.top_p[row], least = set.min_p[row] > 0.f ? fminf(set.min_p[row], 1.0f) : 0.f;
+    const int k = k_in > 0 && k_in < V ? k_in : 0;
+    bool arrived = true;
+    if (bulk_n > 0) arrived = mbar_wait(smem_u32(&s.loaded), 0);
+    if (!arrived) atomicExch(&g_draw_error, 1);
+    __syncthreads();
     auto at = [&](int i) { return logit_of(to_float(slice[i - first])); };
+    const T* my_seg = slice + (lo_i - first);
     if (set.penalty) {
         // tokens of the history, each named once: x / penalty where x > 0, x * penalty elsewhere
         const float pen = set.penalty[row];
-        __syncthreads();
         if (pen != 1.0f)
             for (int h = set.hist_off[row] + tid; h < set.hist_off[row + 1]; h += kThreads) {
                 const int i = set.hist_tok[h];
-                if (i < first || i >= min(first + kWarps * seg, V)) continue;
+                if (i < first || i >= first + slice_n) continue;
                 const float x = at(i);
                 slice[i - first] = from_float<T>(x > 0.f ? x / pen : x * pen);
             }
         __syncthreads();
     }
 
-    // ---- the maximum, and the lowest index that has it
-    unsigned best = 0, best_at = 0x7fffffff;
-    __syncwarp();
-    for (int i = lo_i + lane; i < hi_i; i += 32) {
-        const unsigned k = key_of(at(i));
-        if (k > best) {
-            best = k;
-            best_at = i;
-        }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned k = __shfl_xor_sync(0xffffffffu, best, o), j = __shfl_xor_sync(0xffffffffu, best_at, o);
-        if (k > best || (k == best && j < best_at)) {
-            best = k;
-            best_at = j;
-        }
-    }
-    if (lane == 0) {
-        s.key[warp] = best;
-        s.at[warp] = best_at;
-    }
+    // ---- the maximum; and a key that at least k logits of the row reach, by the largest logits of warps or threads
+    float mx = -INFINITY;
+    each_logit(my_seg, mine_n, lane, [&](int, float x) { mx = fmaxf(mx, x); });      // (NaN counts as -inf)
+    const unsigned mx_key = key_of(mx + 0.0f);
+    const unsigned warp_top = __reduce_max_sync(0xffffffffu, mx_key);
+    if (lane == 0) s.key[warp] = warp_top;
+    unsigned floor_key = 0;
+    const int r = (k + static_cast<int>(ranks) - 1) / static_cast<int>(ranks);
     __syncthreads();
-    if (tid < static_cast<int>(ranks)) {
-        for (int w = 0; w < kWarps; ++w)
-            if (w == 0 || s.key[w] > best || (s.key[w] == best && s.at[w] < best_at)) {
-                best = s.key[w];
-                best_at = s.at[w];
+    if (k > 0 && heat_in > 0.f) {
+        if (r <= kWarps) {
+            // (of the warps' maxima, where these are enough)
+            const unsigned mine = s.key[lane & (kWarps - 1)];
+            int larger = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) larger += s.key[w] > mine ? 1 : 0;
+            floor_key = __reduce_min_sync(0xffffffffu, larger < r ? mine : 0xffffffffu);
+        } else if (r <= kThreads) {
+            for (int bit = 31; bit >= 16; --bit) {
+                const unsigned next = floor_key | (1u << bit);
+                if (__syncthreads_count(mx_key >= next) >= r) floor_key = next;
             }
+        }
+    }
+    if (tid < static_cast<int>(ranks)) {
+        unsigned best = 0;
+        for (int w = 0; w < kWarps; ++w) best = max(best, s.key[w]);
         *cluster.map_shared_rank(&s.top_key[rank], tid) = best;
-        *cluster.map_shared_rank(&s.top_at[rank], tid) = best_at;
+        *cluster.map_shared_rank(&s.floor_key[rank], tid) = floor_key;
     }
     cluster.sync();
-    best = 0;
-    for (unsigned r = 0; r < ranks; ++r)
-        if (s.top_key[r] > best) {
-            best = s.top_key[r];
-            best_at = s.top_at[r];
-        }
+    unsigned best = 0;
+    floor_key = 0xffffffffu;
+    for (unsigned c = 0; c < ranks; ++c) {
+        best = max(best, s.top_key[c]);
+        floor_key = min(floor_key, s.floor_key[c]);
+    }
     const float top = value_of(best);
     const long long draw0 = static_cast<long long>(row) * draws;
     if (!(heat_in > 0.f) || top == -INFINITY) {
-        // greedy; a row in which every logit is -inf has no token to draw: token 0, with probability 0
-        if (rank == 0)
+        // greedy: the lowest index of the maximum; a row in which every logit is -inf has no token to draw: token 0,
+        // with probability 0
+        int lowest = 0x7fffffff;
+        each_logit(my_seg, mine_n, lane, [&](int i, float x) { if (x == top) lowest = min(lowest, lo_i + i); });
+        lowest = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(lowest)));
+        if (lane == 0) s.at[warp] = lowest;
+        __syncthreads();
+        if (tid == 0) {
+            unsigned l = 0x7fffffff;
+            for (int w = 0; w < kWarps; ++w) l = min(l, s.at[w]);
+            *cluster.map_shared_rank(&s.top_at[rank], 0) = l;
+        }
+        cluster.sync();
+        if (rank == 0) {
+            unsigned l = 0x7fffffff;
+            for (unsigned c = 0; c < ranks; ++c) l = min(l, s.top_at[c]);
             for (int j = tid; j < draws; j += kThreads) {
-                out[draw0 + j] = top == -INFINITY ? 0 : static_cast<int>(best_at);
+                out[draw0 + j] = top == -INFINITY ? 0 : static_cast<int>(l);
                 if (prob) prob[draw0 + j] = top == -INFINITY ? 0.f : 1.f;
             }
-        cluster.sync();
-        return;
+        }
+        return;                              // (nobody reads another CTA's memory any more)
     }
     Heat heat;
     heat.top = top;
     heat.c = 1.4426950408889634074 / static_cast<double>(heat_in);
-    heat.bins = static_cast<float>(kBins - 1) / (30.5f * heat_in);
+    heat.bins = 1.0f / (30.5f * heat_in);
+    heat.low = top - 60.0f * heat_in;        // (weights vanish from 30.5 temperatures on)
+    heat.plain = heat_in > 1e-30f && heat_in < 1e30f && fabsf(top) * 2.4e-7f < heat_in;      // (so `low` lies 87 octaves below)
+    heat.powers = s.powers + (lane & (kCopies - 1));
+    const double bound = least > 0.f ? static_cast<double>(least) * static_cast<double>(1ull << kFraction) : 0.0;
 
-    // ---- what is kept: keys above cut_key, and logits equal to it up to index tie_cut
-    unsigned cut_key = 0;
-    int tie_cut = 0x7fffffff, level = 0;
-    u64 ties = 0, ties_kept = 0;
-    const int k = set.top_k[row];
-    if (k > 0 && k < V) {
-        const Cut c = find_cut<false>(cluster, s, heat, at, lo_i, hi_i, 0u, static_cast<u64>(k - 1), level);
-        cut_key = c.key;
-        ties = c.mass;
-        ties_kept = min(ties, static_cast<u64>(k) - c.above);
-    }
-    const float p = set.top_p[row];
-    if (p < 1.0f) {
-        u64 mine = 0;
-        for (int i = lo_i + lane; i < hi_i; i += 32) {
-            const float x = at(i);
-            const unsigned key = key_of(x);
-            if (key > cut_key || (key == cut_key && ties == ties_kept)) mine += heat.weight(x);
-        }
+    // the sum of `mine` over all warps of the cluster
+    auto cluster_sum = [&](u64 mine, u64* exchange) {
         mine = warp_sum64(mine);
         if (lane == 0) s.warp_sum[warp] = mine;
         __syncthreads();
         if (tid < static_cast<int>(ranks)) {
             u64 sum = 0;
             for (int w = 0; w < kWarps; ++w) sum += s.warp_sum[w];
-            *cluster.map_shared_rank(&s.mass[rank], tid) = sum;
+            *cluster.map_shared_rank(&exchange[rank], tid) = sum;
         }
         cluster.sync();
         u64 z = 0;
-        for (unsigned r = 0; r < ranks; ++r) z += s.mass[r];
-        const u64 w_cut = heat.weight(value_of(cut_key));
-        if (ties != ties_kept) z += ties_kept * w_cut;
-        const u64 target = static_cast<u64>(static_cast<double>(fmaxf(p, 0.f)) * static_cast<double>(z));
-        const Cut c = find_cut<true>(cluster, s, heat, at, lo_i, hi_i, cut_key, target, level);
+        for (unsigned c = 0; c < ranks; ++c) z += exchange[c];
+        return z;
+    };
+    bool cut_known = false;                  // top-p's, in s.cut_key and s.tie_cut
+    const bool filtered = k > 0 || p < 1.0f || bound > 0.0;
+    // ---- top-p over the whole row: its mass, and the bin of its cut
+    u64 whole = 0, bin_above = 0, target = 0;
+    unsigned bin_lo = 0, bin_hi = 0;
+    if (k == 0 && p < 1.0f) {
+        // exact sums by 32-bit additions: a weight in three pieces of 15 bits (fewer than 2^17 of them a bin and CTA), most of
+        // which are nothing
+        for (int i = tid; i < 3 * kMassBins; i += kThreads) (&s.pieces[0][0])[i] = 0;
+        if (tid == 0) s.cross_bin = -1;
+        __syncthreads();
+        each_logit(my_seg, mine_n, lane, [&](int, float x) {
+            const u64 w = heat.weight(x);    // (NaN: none)
+            if (!w) return;
+            const int bin = heat.bin<kMassBins>(x);
+            const unsigned a = static_cast<unsigned>(w) & 32767u, b = static_cast<unsigned>(w >> 15) & 32767u, c = static_cast<unsigned>(w >> 30);
+            if (a) atomicAdd(&s.pieces[0][bin], a);
+            if (b) atomicAdd(&s.pieces[1][bin], b);
+            if (c) atomicAdd(&s.pieces[2][bin], c);
+        });
+        cluster.sync();
+        // a CTA adds its share of the bins up, then all of them learn each share's mass, then where the cut lies
+        constexpr int EACH = kMassBins / kThreads;
+        const int share = kMassBins / static_cast<int>(ranks);       // (128 to 2,048)
+        u64 m[EACH] = {}, sum_m = 0;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int bin = EACH * tid + e;
+            if (bin < share)
+                for (unsigned c = 0; c < ranks; ++c) {
+                    const unsigned* other = cluster.map_shared_rank(&s.pieces[0][0], c) + rank * share + bin;
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) m[e] += static_cast<u64>(other[q * kMassBins]) << (15 * q);
+                }
+            sum_m += m[e];
+        }
+        u64 here;
+        const u64 incl = block_scan64(sum_m, s.scan, here);
+        if (tid < static_cast<int>(ranks)) *cluster.map_shared_rank(&s.total[rank], tid) = here;
+        cluster.sync();
+        u64 in_front = 0, of_the_cut = 0;
+        for (unsigned c = 0; c < ranks; ++c) whole += s.total[c];
+        target = static_cast<u64>(static_cast<double>(fmaxf(p, 0.f)) * static_cast<double>(whole));
+        int owner = -1;                      // the last share that has some mass and no more than the target in front of it
+        for (unsigned c = 0; c < ranks; ++c) {
+            if (s.total[c] && in_front <= target) {
+                owner = static_cast<int>(c);
+                of_the_cut = in_front;
+            }
+            in_front += s.total[c];
+        }
+        if (owner == static_cast<int>(rank)) {
+            u64 in_front_of = of_the_cut + incl - sum_m;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                if (m[e] && in_front_of <= target) atomicMax(&s.cross_bin, EACH * tid + e);
+                in_front_of += m[e];
+            }
+            __syncthreads();
+            const int cross = s.cross_bin;   // (>= 0: the share's first bin with mass qualifies)
+            in_front_of = of_the_cut + incl - sum_m;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                if (EACH * tid + e == cross) s.cross_above = in_front_of;
+                in_front_of += m[e];
+            }
+            if (warp == 0) {
+                unsigned lo = 0, hi = best;
+                keys_of_bin<kMassBins>(heat, static_cast<int>(rank) * share + cross, lane, lo, hi);
+                if (lane == 0) {
+                    s.lo = lo;
+                    s.hi = hi;
+                }
+            }
+            __syncthreads();
+            const unsigned found_lo = s.lo, found_hi = s.hi;
+            const u64 found = s.cross_above;
+            __syncthreads();
+            if (tid < static_cast<int>(ranks)) {
+                *cluster.map_shared_rank(&s.lo, tid) = found_lo;
+                *cluster.map_shared_rank(&s.hi, tid) = found_hi;
+                *cluster.map_shared_rank(&s.cross_above, tid) = found;
+            }
+        }
+        cluster.sync();                      // (nobody reads the pieces any more)
+        bin_lo = s.lo;
+        bin_hi = s.hi == 0x7fffffffu ? s.hi - 1 : s.hi;      // (the key of -0, which no logit has: as a float it equals 0)
+        bin_above = s.cross_above;
+    }
+    if (filtered) {
+        // ---- what can be kept at all: keys from floor_key on
+        if (k == 0) floor_key = bin_lo;      // (0 without top-p)
+        if (bound > 0.0 && (k == 0 || p >= 1.0f)) {
+            if (warp == 0) {
+                const unsigned lowest = first_key(key_of(-INFINITY), best, lane, [&](unsigned q) { return heat.scaled(value_of(q)) >= bound; });
+                if (lane == 0) s.key[0] = lowest;
+            }
+            __syncthreads();
+            floor_key = max(floor_key, s.key[0]);
+            __syncthreads();
+        }
+        // counted and listed: the survivors, and where top-p's bin is known its tokens (x, y)
+        const unsigned bin_top = k == 0 && p < 1.0f ? bin_hi : 0u;
+        uint2 mine = make_uint2(0, 0);
+        const bool take_all = floor_key <= key_of(-INFINITY);        // (NaN, too)
+        const float floor_x = value_of(max(floor_key, key_of(-INFINITY)));
+        const float bin_lo_x = bin_top ? value_of(max(bin_lo, key_of(-INFINITY))) : INFINITY, bin_hi_x = bin_top ? value_of(bin_hi) : -INFINITY;
+        auto in_all = [&](float x) { return x >= floor_x || take_all; };
+        auto in_bin = [&](float x) { return x >= bin_lo_x && x <= bin_hi_x; };      // (not NaN: it has no weight)
+        each_logit(my_seg, mine_n, lane, [&](int, float x) {
+            mine.x += in_all(x) ? 1u : 0u;
+            mine.y += in_bin(x) ? 1u : 0u;
+        });
+        mine.x = __reduce_add_sync(0xffffffffu, mine.x);
+        mine.y = __reduce_add_sync(0xffffffffu, mine.y);
+        if (lane == 0) {
+            s.key[warp] = mine.x;
+            s.at[warp] = mine.y;
+        }
+        __syncthreads();
+        uint2 before = make_uint2(0, 0), here = make_uint2(0, 0);
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) {
+                before.x += s.key[w];
+                before.y += s.at[w];
+            }
+            here.x += s.key[w];
+            here.y += s.at[w];
+        }
+        const bool list_all = here.x <= kListed, list_bin = here.y <= kListed;
+        if ((list_all && mine.x) || (list_bin && mine.y)) {
+            // in the order of indices
+            for (int i0 = 0; i0 < mine_n; i0 += 128) {
+                float x[4];
+                bool in = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = i0 + 32 * e + lane;
+                    x[e] = i < mine_n ? to_float(my_seg[i]) : 0.f;
+                    in = in || (i < mine_n && (in_all(x[e]) || in_bin(x[e])));
+                }
+                if (!__any_sync(0xffffffffu, in)) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = i0 + 32 * e + lane;
+                    const Token token{key_of(logit_of(x[e])), lo_i + i};
+                    if (list_all) {
+                        const bool hit = i < mine_n && in_all(x[e]);
+                        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+                        if (hit) s.list[before.x + __popc(hits & ((1u << lane) - 1))] = token;
+                        before.x += __popc(hits);
+                    }
+                    if (list_bin) {
+                        const bool hit = i < mine_n && in_bin(x[e]);
+                        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+                        if (hit) s.bin_list[before.y + __popc(hits & ((1u << lane) - 1))] = token;
+                        before.y += __popc(hits);
+                    }
+                }
+            }
+        }
+        if (tid < static_cast<int>(ranks)) *cluster.map_shared_rank(&s.listed[rank], tid) = here;
+        cluster.sync();
+        unsigned n = 0, n_bin = 0;
+        for (unsigned c = 0; c < ranks; ++c) {
+            n += s.listed[c].x;              // (fewer than 2^20 together)
+            n_bin += s.listed[c].y;
+        }
+        // all of them in the first CTA, in the order of indices
+        auto gather = [&](bool bins, unsigned count) {
+            for (unsigned i = tid; rank == 0 && i < count; i += kThreads) {
+                unsigned c = 0, from = 0;
+                for (unsigned end = bins ? s.listed[0].y : s.listed[0].x; i >= end; end += bins ? s.listed[c].y : s.listed[c].x) {
+                    from = end;
+                    ++c;
+                }
+                const Token* other = bins ? cluster.map_shared_rank(s.bin_list, c) : cluster.map_shared_rank(s.list, c);
+                s.all[i] = other[i - from];
+            }
+        };
+        if (n > kListed && bin_top && n_bin <= kListed) {
+            // ---- the first CTA finds top-p's cut among the tokens of its bin
+            gather(true, n_bin);
+            if (rank == 0) {
+                __syncthreads();
+                for (int i = tid; i < static_cast<int>(n_bin); i += kThreads)
+                    s.order[i] = (static_cast<u64>(s.all[i].key) << 32) | (0xffffffffu - i);
+                __syncthreads();
+                sort_descending(s.order, static_cast<int>(n_bin));
+                u64 w[2], sum;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    w[e] = 2 * tid + e < static_cast<int>(n_bin) ? heat.weight(value_of(static_cast<unsigned>(s.order[2 * tid + e] >> 32))) : 0ull;
+                const u64 incl = block_scan64(w[0] + w[1], s.scan, sum);
+                const int kept = __syncthreads_count(w[0] && bin_above + incl - w[0] - w[1] <= target) +
+                                 __syncthreads_count(w[1] && bin_above + incl - w[1] <= target);
+                if (tid < static_cast<int>(ranks)) {
+                    const Token last = s.all[0xffffffffu - static_cast<unsigned>(s.order[max(kept, 1) - 1])];
+                    *cluster.map_shared_rank(&s.cut_key, tid) = last.key;
+                    *cluster.map_shared_rank(&s.tie_cut, tid) = last.at;
+                }
+            }
+            cluster.sync();
+            cut_known = true;
+        }
+        if (n <= kListed) {
+            // ---- the first CTA takes it from here
+            gather(false, n);
+            cluster.sync();                  // (the others' lists have been read)
+            if (rank != 0) return;
+            for (int i = tid; i < static_cast<int>(n); i += kThreads)
+                s.order[i] = (static_cast<u64>(s.all[i].key) << 32) | (0xffffffffu - i);
+            __syncthreads();
+            sort_descending(s.order, static_cast<int>(n));
+            // weights by value, two a thread; what top-k leaves
+            const int nk = k > 0 ? min(k, static_cast<int>(n)) : static_cast<int>(n);
+            double scaled[2];
+            u64 w[2];
+            int place[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int i = 2 * tid + e;
+                const u64 o = i < nk ? s.order[i] : 0ull;
+                scaled[e] = i < nk ? heat.scaled(value_of(static_cast<unsigned>(o >> 32))) : 0.0;
+                w[e] = i < nk ? heat.weight(value_of(static_cast<unsigned>(o >> 32))) : 0ull;
+                place[e] = i < nk ? static_cast<int>(0xffffffffu - static_cast<unsigned>(o)) : -1;
+            }
+            u64 sum;
+            const u64 incl = block_scan64(w[0] + w[1], s.scan, sum);
+            const u64 z_top = k > 0 ? sum : whole;
+            target = static_cast<u64>(static_cast<double>(fmaxf(p, 0.f)) * static_cast<double>(z_top));
+            for (int i = tid; i < static_cast<int>(n); i += kThreads) s.weight[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const u64 front = e == 0 ? incl - w[0] - w[1] : incl - w[1];
+                if (place[e] >= 0 && (!(p < 1.0f) || front <= target) && scaled[e] >= bound) s.weight[place[e]] = w[e];
+            }
+            __syncthreads();
+            // cumulated in the order of indices
+            u64 z, c2[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) c2[e] = 2 * tid + e < static_cast<int>(n) ? s.weight[2 * tid + e] : 0ull;
+            const u64 incl2 = block_scan64(c2[0] + c2[1], s.scan, z);
+            if (2 * tid < static_cast<int>(n)) s.weight[2 * tid] = incl2 - c2[1];
+            if (2 * tid + 1 < static_cast<int>(n)) s.weight[2 * tid + 1] = incl2;
+            __syncthreads();
+            for (int j = tid; j < draws; j += kThreads) {
+                const u64 goal = drawn_mass(uniform[draw0 + j], z);
+                int lo = 0, hi = static_cast<int>(n) - 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s.weight[mid] > goal) hi = mid;
+                    else lo = mid + 1;
+                }
+                out[draw0 + j] = s.all[lo].at;
+                if (prob) prob[draw0 + j] = static_cast<float>(heat.scaled(value_of(s.all[lo].key)) / static_cast<double>(z));
+            }
+            return;
+        }
+    }
+
+    // ---- no filter, or too many survivors for one CTA: what is kept is keys above cut_key, and logits equal to it up to
+    // index tie_cut
+    unsigned cut_key = 0;
+    int tie_cut = 0x7fffffff, level = 0;
+    u64 ties = 0, ties_kept = 0;
+    if (k > 0) {
+        const Cut c = find_cut<false>(cluster, s, heat, at, lo_i, hi_i, 0u, best, 0ull, false, static_cast<u64>(k - 1), level);
+        cut_key = c.key;
+        ties = c.mass;
+        ties_kept = min(ties, static_cast<u64>(k) - c.above);
+    }
+    if (cut_known) {
+        cut_key = s.cut_key;
+        tie_cut = s.tie_cut;
+    } else if (p < 1.0f) {
+        u64 z = whole;
+        if (k > 0) {
+            u64 mine = 0;
+            for (int i = lo_i + lane; i < hi_i; i += 32) {
+                const float x = at(i);
+                const unsigned key = key_of(x);
+                if (key > cut_key || (key == cut_key && ties == ties_kept)) mine += heat.weight(x);
+            }
+            z = cluster_sum(mine, s.mass);
+            if (ties != ties_kept) z += ties_kept * heat.weight(value_of(cut_key));
+        }
+        target = static_cast<u64>(static_cast<double>(fmaxf(p, 0.f)) * static_cast<double>(z));
+        const Cut c = k > 0 ? find_cut<true>(cluster, s, heat, at, lo_i, hi_i, cut_key, best, 0ull, false, target, level)
+                            : find_cut<true>(cluster, s, heat, at, lo_i, hi_i, bin_lo, bin_hi, bin_above, true, target, level);
         const u64 w = heat.weight(value_of(c.key));
         const u64 there = c.key == cut_key && ties ? ties_kept : c.mass / w;    // tokens of that key which top-k left
         const u64 all = c.key == cut_key && ties ? ties : there;
@@ -345,10 +796,8 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         ties = all;
         ties_kept = min(there, (target - c.above) / w + 1);
     }
-    const float least = fminf(set.min_p[row], 1.0f);
-    if (least > 0.f) {
+    if (bound > 0.0) {
         // the smallest key whose weight is min-p of the largest
-        const double bound = static_cast<double>(least) * static_cast<double>(1ull << kFraction);
         if (warp == 0) {
             const unsigned lowest = first_key(key_of(-INFINITY), best, lane, [&](unsigned q) { return heat.scaled(value_of(q)) >= bound; });
             if (lane == 0) s.lo = lowest;
@@ -357,6 +806,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         if (s.lo > cut_key) {
             cut_key = s.lo;
             ties = ties_kept = 0;
+            tie_cut = 0x7fffffff;
         }
     }
     if (ties_kept < ties) {
@@ -364,6 +814,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         unsigned mine = 0;
         for (int i = lo_i + lane; i < hi_i; i += 32) mine += key_of(at(i)) == cut_key ? 1u : 0u;
         mine = __reduce_add_sync(0xffffffffu, mine);
+        __syncthreads();
         if (lane == 0) s.key[warp] = mine;
         __syncthreads();
         if (tid < static_cast<int>(ranks)) {
@@ -373,7 +824,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         }
         cluster.sync();
         u64 before = 0;
-        for (unsigned r = 0; r < rank; ++r) before += s.ties[r];
+        for (unsigned c = 0; c < rank; ++c) before += s.ties[c];
         for (int w = 0; w < warp; ++w) before += s.key[w];
         // (tie_cut is this warp's own: all of its tokens in front of the last kept tie, behind it none)
         if (before >= ties_kept) {
@@ -391,55 +842,48 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
             }
         }
     }
-    auto kept_weight = [&](int i) -> u64 {
-        const float x = at(i);
+    auto kept_weight = [&](int i, float raw) -> u64 {
+        const float x = logit_of(raw);
         const unsigned key = key_of(x);
         return key > cut_key || (key == cut_key && i <= tie_cut) ? heat.weight(x) : 0ull;
     };
 
-    // ---- masses of the segments
+    // ---- masses: a lane's are those of a contiguous block of its warp's segment (an odd number of tokens: no two lanes
+    // of a warp in one bank)
+    const int block_n = ((seg + 31) / 32) | 1;
+    const int b0 = min(lane * block_n, mine_n), b1 = min(b0 + block_n, mine_n);
     u64 mine = 0;
-    for (int i = lo_i + lane; i < hi_i; i += 32) mine += kept_weight(i);
-    mine = warp_sum64(mine);
-    __syncthreads();
-    if (lane == 0) s.warp_sum[warp] = mine;
-    __syncthreads();
-    if (tid < static_cast<int>(ranks)) {
-        u64 sum = 0;
-        for (int w = 0; w < kWarps; ++w) sum += s.warp_sum[w];
-        *cluster.map_shared_rank(&s.total[rank], tid) = sum;
-    }
-    cluster.sync();
-    u64 z = 0, base_mass = 0;
-    for (unsigned r = 0; r < ranks; ++r) {
-        if (r == rank) base_mass = z;
-        z += s.total[r];
-    }
-    // ---- the draws: a draw whose number falls on this CTA is taken by the warp on whose segment it falls
-    u64 from = base_mass;
+    for (int i = b0; i < b1; ++i) mine += kept_weight(lo_i + i, to_float(my_seg[i]));
+    __syncthreads();                         // (warp_sum may still be read)
+    const u64 z = cluster_sum(mine, s.total);
+    u64 from = 0;
+    for (unsigned c = 0; c < rank; ++c) from += s.total[c];
     for (int w = 0; w < warp; ++w) from += s.warp_sum[w];
+    from += warp_scan64(mine, lane) - mine;  // what lies in front of this lane's block
+    // ---- the draws: each is taken by the warp on whose segment its number falls
     for (int j = 0; j < draws; ++j) {
-        const float u = uniform[draw0 + j];
-        u64 target = u > 0.f ? static_cast<u64>(static_cast<double>(u) * static_cast<double>(z)) : 0ull;
-        target = min(target, z - 1);
-        if (target < from || target >= from + mine) continue;
-        u64 sum = from;
-        for (int base = lo_i; base < hi_i; base += 32) {
-            const u64 w = base + lane < hi_i ? kept_weight(base + lane) : 0ull;
+        const u64 goal = drawn_mass(uniform[draw0 + j], z);
+        const unsigned owner = __ballot_sync(0xffffffffu, goal >= from && goal < from + mine);
+        if (!owner) continue;
+        const int l = __ffs(owner) - 1;
+        u64 sum = __shfl_sync(0xffffffffu, from, l);
+        const int first_of = l * block_n, end_of = min(first_of + block_n, mine_n);
+        for (int base = first_of; base < end_of; base += 32) {
+            const int i = base + lane;
+            const u64 w = i < end_of ? kept_weight(lo_i + i, to_float(my_seg[i])) : 0ull;
             const u64 incl = warp_scan64(w, lane) + sum;
-            const unsigned over = __ballot_sync(0xffffffffu, incl > target);
+            const unsigned over = __ballot_sync(0xffffffffu, incl > goal);
             if (over) {
-                const int l = __ffs(over) - 1;
-                if (lane == l) {
-                    out[draw0 + j] = base + lane;
-                    if (prob) prob[draw0 + j] = static_cast<float>(heat.scaled(at(base + lane)) / static_cast<double>(z));
+                if (lane == __ffs(over) - 1) {
+                    out[draw0 + j] = lo_i + i;
+                    if (prob) prob[draw0 + j] = static_cast<float>(heat.scaled(at(lo_i + i)) / static_cast<double>(z));
                 }
                 break;
             }
             sum = __shfl_sync(0xffffffffu, incl, 31);
         }
     }
-    cluster.sync();                          // no CTA leaves while another may still read its histograms
+    // (nobody reads another CTA's memory behind the last sum: all may leave)
 }
 
 template <typename T>
@@ -447,7 +891,7 @@ int launch_draw(const void* logits, long long stride, int rows, int V, const Set
                 int* out, float* prob, cudaStream_t stream) {
     int ranks = 1;
     while (ranks < 8 && V > ranks * 4096) ranks *= 2;
-    const int most = 200 * 1024;             // bytes of a slice beside the static shared memory
+    const int most = 192 * 1024;             // bytes of a slice beside the static shared memory
     const auto segment = [&](int n) { return ((V + n * kWarps - 1) / (n * kWarps) + 7) / 8 * 8; };
     while (ranks < kMaxCluster && static_cast<long long>(segment(ranks)) * kWarps * sizeof(T) > most) ranks *= 2;
     const int seg = segment(ranks);
@@ -465,6 +909,13 @@ int launch_draw(const void* logits, long long stride, int rows, int V, const Set
 }  // namespace somi
 
 using namespace somi;
+
+SOMI_API int somi_draw_error() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, draw::g_draw_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(draw::g_draw_error, &zero, sizeof(int));
+    return v;
+}
 
 // logits [rows, V] (rows `stride` elements apart), uniform, out and prob (or null) [rows, draws]; temperature, top_k,
 // top_p, min_p [rows]; penalty [rows], hist_off [rows + 1] and hist_tok, or all null (float32 logits only).

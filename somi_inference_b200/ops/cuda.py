@@ -344,6 +344,8 @@ class CudaOps:
         if int(self.lib.somi_shared_attention_error()) != 0:
             raise KernelError("the tcgen05 attention over shared prefixes gave up waiting on a barrier; "
                               "its results are not valid")
+        if int(self.lib.somi_draw_error()) != 0:
+            raise KernelError("draw_tokens gave up waiting for a copy of its logits; its tokens are not valid")
         if int(self.lib.somi_chunks_error()) != 0:
             raise KernelError("the recurrence in chunks gave up waiting on a barrier; "
                               "its results are not valid")

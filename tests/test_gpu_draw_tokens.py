@@ -72,6 +72,26 @@ def test_flat_rows(ops, dtype):
     check(ops, x, [(50.0, k, p, m) for _, k, p, m in SETTINGS], u)
 
 
+def test_a_mass_cut_among_a_whole_vocabulary(ops):
+    """top-p alone, its cut among tens of thousands of kept tokens; zeros, masked and NaN logits among them, several maxima."""
+    g = torch.Generator().manual_seed(30)
+    x = torch.randn(10, 60001, generator=g)
+    x[1, ::3] = 0.0
+    x[1, 1::3] = -0.0
+    x[2, ::2] = float("nan")
+    x[3, ::2] = -float("inf")
+    x[4] = (x[4] * 4).round() / 4            # few different values
+    x[5] *= 12                               # most of the mass in a few, the cut in what vanishes
+    x[6, 100:110] = 9.0
+    x[7] = x[7].abs() * -1e-3
+    x[8] = torch.linspace(-40, 0, 60001)[torch.randperm(60001, generator=g)]
+    u = torch.rand(10, 20, generator=g)
+    for dtype in (torch.float32, torch.bfloat16):
+        for p in (0.5, 0.95, 0.999999):
+            check(ops, x.to(dtype), [(1.0, -1, p, 0.0), (0.9, -1, p, 0.0), (1.0, 0, p, 0.2), (1.0, 70000, p, 0.0), (1.0, -1, p, 1e-3)] * 2, u)
+    ops.check_errors()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_equal_logits_are_kept_by_their_index(ops, dtype):
     """Few different values, so every cut lies among equal ones: 3 values, and all equal."""
