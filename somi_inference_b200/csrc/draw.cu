@@ -7,29 +7,32 @@
 //     draw: the first i in index order whose cumulated mass over kept tokens is above u (kept mass)
 //
 // Which token a number falls on, and where a cut lies, is a comparison of sums, so these must not depend
-// on the order of summation nor on float32's rounding: a weight is computed to 2^-37 of itself (`Heat::weight`)
-// and held as an integer multiple of 2^-44, and sums of integers are exact.  (Fewer than 2^20 weights of at most 2^44 stay below 2^64.)  So the result is the same bits
-// whatever the launch looks like, and differs from real arithmetic only where a border lies within
-// about 1e-11 of the number.
+// on the order of summation nor on float32's rounding: a weight is computed in float64 (2^r by its Taylor
+// series, relative error 3e-16) and held as an integer multiple of 2^-44, and sums of integers are exact.
+// (Fewer than 2^20 weights of at most 2^44 stay below 2^64.)  So the result is the same bits whatever the launch
+// looks like, and differs from real arithmetic only where a border lies within about 1e-11 of the number.
 //
 // A cluster of CTAs shares a row; each holds its slice in shared memory, read from HBM once, as a bulk copy where
 // the row is aligned.  A warp owns a contiguous segment of it.  All three cuts keep a beginning of one order, so a
 // token can be left out as soon as it is known to lie behind a cut:
 //     top-k: the r-th largest of a CTA's warps' (or threads') maxima, r = k / (CTAs of the cluster), has r logits at or above
 //            it in that CTA, so the least such value of the cluster has k at or above it in the row;
-//     top-p: the masses of 1,024 bins of the logits' distance from the maximum say in which bin the cut lies;
+//     top-p: the masses of 2,048 bins of the logits' distance from the maximum say in which bin the cut lies;
 //     min-p: by its definition.
-// What is left (the survivors, in the order of their indices) is usually a few dozen to a few hundred tokens; they are collected in one
-// CTA, sorted, cut and drawn from there: a row of 152,064 logits costs a pass for its maximum and one that
+// What is left (the survivors, in the order of their indices) is usually a few dozen to a few hundred tokens; they are
+// collected in one CTA, sorted, cut and drawn from there: a row of 152,064 logits costs a pass for its maximum and one that
 // looks for survivors, and only a row with top-p and without top-k a weight for every token.  Where more than
 // `kListed` survive, the cuts are found by histograms that the cluster's CTAs add up: first those bins (they
 // span the 30.5 temperatures in which weights do not vanish), then the keys (the order-preserving integer image of a
-// float) that lie in the bin of the cut, until a bin is one key; what is kept is then a key and an index up to which logits equal to it are
-// kept, and weights are computed a second time to find where the numbers fall.
+// float) that lie in the bin of the cut, until a bin is one key (top-p's bin, where it holds no more than `kListed`,
+// is sorted in one CTA instead); what is kept is then a key and an index up to which logits equal to it are kept, and
+// weights are computed a second time to find where the numbers fall.
 #include <cooperative_groups.h>
 
-#include "tma.cuh"
+#include <algorithm>
+
 #include "mma.cuh"
+#include "tma.cuh"
 
 namespace somi {
 namespace draw {
@@ -38,9 +41,9 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kMaxCluster = 16;
 constexpr int kMassBins = 2048;              // of the masses that top-p cuts
-constexpr int kListed = 1024;                // survivors that one CTA takes
+constexpr int kListed = 2048;                // survivors that one CTA takes
+constexpr int kBinListed = 1024;             // tokens of top-p's bin that one CTA takes
 constexpr int kFraction = 44;                // a weight is an integer multiple of 2^-44
-constexpr int kCopies = 16;                  // of the table of powers
 typedef unsigned long long u64;
 
 struct Settings {
@@ -52,23 +55,19 @@ struct Token { unsigned key; int at; };
 
 struct Shared {
     union {
+        u64 hist[2][kBins];                  // (read by the other CTAs of the cluster)
+        unsigned pieces[3][kMassBins];       // masses of bins in pieces of 15 bits (likewise)
         struct {
             union {
-                u64 hist[2][kBins];          // (read by the other CTAs of the cluster)
-                struct {
-                    Token list[kListed];     // this CTA's survivors (read by the first CTA)
-                    Token bin_list[kListed]; // its tokens of the cut's bin (likewise)
-                };
-                struct {
-                    u64 order[kListed];      // in the first CTA: all of them by value,
-                    u64 weight[kListed];     // and their weights
+                Token list[kListed];         // this CTA's survivors (likewise)
+                struct {                     // in the first CTA, where it cuts top-p's bin:
+                    u64 bin_order[kBinListed];       // the tokens by value,
+                    Token bin_all[kBinListed];       // and in the order of indices
                 };
             };
-            Token all[kListed];              // the first CTA: the row's survivors
+            Token bin_list[kBinListed];      // this CTA's tokens of top-p's bin (likewise)
         };
-        unsigned pieces[3][kMassBins];       // masses of bins in pieces of 15 bits (read by the other CTAs)
     };
-    u64 powers[64 * kCopies];
     u64 scan[kWarps];
     u64 warp_sum[kWarps];
     u64 total[kMaxCluster], mass[kMaxCluster];   // written by the other CTAs, one exchange each
@@ -94,11 +93,17 @@ __device__ __forceinline__ float value_of(unsigned key) {
 // A logit: NaN counts as -inf, -0 as 0 (equal values must have equal keys).
 __device__ __forceinline__ float logit_of(float x) { return x == x ? x + 0.0f : -INFINITY; }
 
-// 2^r = 1 + r ln 2 (1 + r ln 2 / 2 (1 + r ln 2 / 3 (...))), to the N-th power of r (|r| <= 1/2, N = 13: 2e-16)
+// ln(2)^K / K!
+template <int K>
+struct Taylor { static constexpr double value = Taylor<K - 1>::value * 0.69314718055994530942 / K; };
+template <>
+struct Taylor<0> { static constexpr double value = 1.0; };
+
+// 2^r by the first N + 1 terms of its Taylor series, |r| <= 1/2 (N = 12: 2e-16)
 template <int N, int K = 0>
 __device__ __forceinline__ double exp2_taylor(double r) {
-    if constexpr (K == N) return 1.0;
-    else return fma(exp2_taylor<N, K + 1>(r), r * (0.69314718055994530942 / (K + 1)), 1.0);
+    if constexpr (K == N) return Taylor<K>::value;
+    else return fma(exp2_taylor<N, K + 1>(r), r, Taylor<K>::value);
 }
 
 // A row's maximum and temperature: what a weight depends on.
@@ -106,42 +111,24 @@ struct Heat {
     float top;
     double c;                                // log2(e) / T
     float bins;                              // 1 / the distance from the maximum at which bins end
-    float low;                               // below it every weight is nothing
-    const u64* powers;                       // 2^(62 + j / 64) at kCopies j, j = 0 .. 63: this lane's copy
-    bool plain;                              // the maximum is not so large that its neighbours have no weight
 
-    // w 2^44 before it is rounded to an integer; 0 where w < 2^-44
+    // w 2^44 before it is rounded to an integer; 0 where w < 2^-44.  NaN and -inf have no weight.  (float64 throughout: its
+    // pipe takes a warp's operation in two cycles, and what integers and tables did instead took twice as long.)
     __device__ __forceinline__ double scaled(float x) const {
-        if (x == top) return static_cast<double>(1ull << kFraction);
         const double y = (static_cast<double>(x) - static_cast<double>(top)) * c;
-        if (!(y >= -static_cast<double>(kFraction))) return 0.0;       // (-inf, and inf - inf, too)
         const double magic = 6755399441055744.0;                      // 1.5 2^52: adding it rounds to an integer
         const double shifted = y + magic;
-        const double r = y - (shifted - magic);
-        const int n = static_cast<int>(__double_as_longlong(shifted));  // (the low bits)
-        const double p = exp2_taylor<13>(r);
-        return __longlong_as_double(__double_as_longlong(p) + (static_cast<long long>(n + kFraction) << 52));
+        const double p = exp2_taylor<12>(y - (shifted - magic));
+        const int n = __double2loint(shifted) + kFraction;
+        const double w = __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+        if (top == INFINITY) return x == top ? static_cast<double>(1ull << kFraction) : 0.0;      // (of several: equal)
+        return y >= -static_cast<double>(kFraction) ? w : 0.0;         // (else `w` may be anything)
     }
-    // The integer.  float64 operations are rare here (16 a cycle and SM): three of them make y = (x - max) c + 1536, whose
-    // low 42 bits are the fraction of y, the next ten 512 + its floor; 2^fraction is a table's value for six bits times
-    // 1 + r a1 + .. + r^4 a4, r below 2^-6 and held to 2^-38, in 32-bit integers (a_k = ln(2)^k / k!).  Relative error at
-    // most 2^-37.  The table has a copy for every two lanes of a warp, since lanes that read different entries of one copy
-    // meet in the same banks.
-    __device__ __forceinline__ u64 weight(float x) const {
-        if (!plain) return static_cast<u64>(__double_as_longlong(scaled(logit_of(x)) + 4503599627370496.0)) & ((1ull << 52) - 1);
-        const double d = static_cast<double>(fmaxf(x, low)) - static_cast<double>(top);
-        const double v = fma(d, c, 1536.0);
-        const unsigned hi = static_cast<unsigned>(__double2hiint(v));
-        const unsigned r = __funnelshift_r(static_cast<unsigned>(__double2loint(v)), hi, 4);
-        const int n = 512 - static_cast<int>((hi >> 10) & 1023u);      // -floor(y)
-        const u64 t = powers[((hi >> 4) & 63u) * kCopies];
-        unsigned e = 58200u + __umulhi(r, 158u);                       // a3 2^20, a4 2^14
-        e = 16121328u + __umulhi(r, e);                                // a2 2^26
-        e = 2977044472u + __umulhi(r, e);                              // a1 2^32
-        e = __umulhi(r, e);                                            // (2^(r / 2^38) - 1) 2^38
-        const u64 whole = t + ((static_cast<u64>(static_cast<unsigned>(t >> 32)) * e) >> 6);
-        return n > kFraction ? 0ull : (whole + (1ull << (61 - kFraction + n))) >> (62 - kFraction + n);
+    __device__ __forceinline__ static u64 rounded(double scaled) {
+        const double shifted = scaled + 4503599627370496.0;            // 2^52: the integer is in the low bits
+        return static_cast<u64>(__double_as_longlong(shifted)) & ((1ull << 52) - 1);
     }
+    __device__ __forceinline__ u64 weight(float x) const { return rounded(scaled(x)); }
     // falls (or stays) as x grows
     template <int BINS>
     __device__ __forceinline__ int bin(float x) const {
@@ -382,12 +369,6 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
                      : "memory");
     }
     for (int i = bulk_n + tid; i < slice_n; i += kThreads) slice[i] = x_row[i];
-    // (while the logits are on their way)
-    for (int i = tid; i < 64 * kCopies; i += kThreads) {
-        const int j = i / kCopies;
-        const double t = exp2_taylor<13>((j < 32 ? j : j - 64) * (1.0 / 64.0)) * (j < 32 ? 4611686018427387904.0 : 9223372036854775808.0);
-        s.powers[i] = static_cast<u64>(t);
-    }
     const float heat_in = set.temperature[row];
     const int k_in = set.top_k[row];
     const float p = set.top_p[row], least = set.min_p[row] > 0.f ? fminf(set.min_p[row], 1.0f) : 0.f;
@@ -396,6 +377,10 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
     if (bulk_n > 0) arrived = mbar_wait(smem_u32(&s.loaded), 0);
     if (!arrived) atomicExch(&g_draw_error, 1);
     __syncthreads();
+    // the first CTA's survivors: by value, their weights, and in the order of indices (in its slice's place, once it is done with that)
+    u64* const order = reinterpret_cast<u64*>(slice_raw);
+    u64* const weight_of = order + kListed;
+    Token* const all_of = reinterpret_cast<Token*>(weight_of + kListed);
     auto at = [&](int i) { return logit_of(to_float(slice[i - first])); };
     const T* my_seg = slice + (lo_i - first);
     if (set.penalty) {
@@ -478,9 +463,6 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
     heat.top = top;
     heat.c = 1.4426950408889634074 / static_cast<double>(heat_in);
     heat.bins = 1.0f / (30.5f * heat_in);
-    heat.low = top - 60.0f * heat_in;        // (weights vanish from 30.5 temperatures on)
-    heat.plain = heat_in > 1e-30f && heat_in < 1e30f && fabsf(top) * 2.4e-7f < heat_in;      // (so `low` lies 87 octaves below)
-    heat.powers = s.powers + (lane & (kCopies - 1));
     const double bound = least > 0.f ? static_cast<double>(least) * static_cast<double>(1ull << kFraction) : 0.0;
 
     // the sum of `mine` over all warps of the cluster
@@ -627,7 +609,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
             here.x += s.key[w];
             here.y += s.at[w];
         }
-        const bool list_all = here.x <= kListed, list_bin = here.y <= kListed;
+        const bool list_all = here.x <= kListed, list_bin = here.y <= kBinListed;
         if ((list_all && mine.x) || (list_bin && mine.y)) {
             // in the order of indices
             for (int i0 = 0; i0 < mine_n; i0 += 128) {
@@ -667,7 +649,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
             n_bin += s.listed[c].y;
         }
         // all of them in the first CTA, in the order of indices
-        auto gather = [&](bool bins, unsigned count) {
+        auto gather = [&](bool bins, Token* to, unsigned count) {
             for (unsigned i = tid; rank == 0 && i < count; i += kThreads) {
                 unsigned c = 0, from = 0;
                 for (unsigned end = bins ? s.listed[0].y : s.listed[0].x; i >= end; end += bins ? s.listed[c].y : s.listed[c].x) {
@@ -675,27 +657,27 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
                     ++c;
                 }
                 const Token* other = bins ? cluster.map_shared_rank(s.bin_list, c) : cluster.map_shared_rank(s.list, c);
-                s.all[i] = other[i - from];
+                to[i] = other[i - from];
             }
         };
-        if (n > kListed && bin_top && n_bin <= kListed) {
+        if (n > kListed && bin_top && n_bin <= kBinListed) {
             // ---- the first CTA finds top-p's cut among the tokens of its bin
-            gather(true, n_bin);
+            gather(true, s.bin_all, n_bin);
             if (rank == 0) {
                 __syncthreads();
                 for (int i = tid; i < static_cast<int>(n_bin); i += kThreads)
-                    s.order[i] = (static_cast<u64>(s.all[i].key) << 32) | (0xffffffffu - i);
+                    s.bin_order[i] = (static_cast<u64>(s.bin_all[i].key) << 32) | (0xffffffffu - i);
                 __syncthreads();
-                sort_descending(s.order, static_cast<int>(n_bin));
+                sort_descending(s.bin_order, static_cast<int>(n_bin));
                 u64 w[2], sum;
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    w[e] = 2 * tid + e < static_cast<int>(n_bin) ? heat.weight(value_of(static_cast<unsigned>(s.order[2 * tid + e] >> 32))) : 0ull;
+                    w[e] = 2 * tid + e < static_cast<int>(n_bin) ? heat.weight(value_of(static_cast<unsigned>(s.bin_order[2 * tid + e] >> 32))) : 0ull;
                 const u64 incl = block_scan64(w[0] + w[1], s.scan, sum);
                 const int kept = __syncthreads_count(w[0] && bin_above + incl - w[0] - w[1] <= target) +
                                  __syncthreads_count(w[1] && bin_above + incl - w[1] <= target);
                 if (tid < static_cast<int>(ranks)) {
-                    const Token last = s.all[0xffffffffu - static_cast<unsigned>(s.order[max(kept, 1) - 1])];
+                    const Token last = s.bin_all[0xffffffffu - static_cast<unsigned>(s.bin_order[max(kept, 1) - 1])];
                     *cluster.map_shared_rank(&s.cut_key, tid) = last.key;
                     *cluster.map_shared_rank(&s.tie_cut, tid) = last.at;
                 }
@@ -705,56 +687,64 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         }
         if (n <= kListed) {
             // ---- the first CTA takes it from here
-            gather(false, n);
+            gather(false, all_of, n);
             cluster.sync();                  // (the others' lists have been read)
             if (rank != 0) return;
-            for (int i = tid; i < static_cast<int>(n); i += kThreads)
-                s.order[i] = (static_cast<u64>(s.all[i].key) << 32) | (0xffffffffu - i);
+            const int count = static_cast<int>(n);
+            for (int i = tid; i < count; i += kThreads) order[i] = (static_cast<u64>(all_of[i].key) << 32) | (0xffffffffu - i);
             __syncthreads();
-            sort_descending(s.order, static_cast<int>(n));
-            // weights by value, two a thread; what top-k leaves
-            const int nk = k > 0 ? min(k, static_cast<int>(n)) : static_cast<int>(n);
-            double scaled[2];
-            u64 w[2];
-            int place[2];
+            sort_descending(order, count);
+            // weights by value, kEach a thread; what top-k leaves
+            constexpr int kEach = kListed / kThreads;
+            const int nk = k > 0 ? min(k, count) : count;
+            double scaled[kEach];
+            u64 w[kEach], sum_w = 0;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int i = 2 * tid + e;
-                const u64 o = i < nk ? s.order[i] : 0ull;
-                scaled[e] = i < nk ? heat.scaled(value_of(static_cast<unsigned>(o >> 32))) : 0.0;
-                w[e] = i < nk ? heat.weight(value_of(static_cast<unsigned>(o >> 32))) : 0ull;
-                place[e] = i < nk ? static_cast<int>(0xffffffffu - static_cast<unsigned>(o)) : -1;
+            for (int e = 0; e < kEach; ++e) {
+                const int i = kEach * tid + e;
+                scaled[e] = i < nk ? heat.scaled(value_of(static_cast<unsigned>(order[i] >> 32))) : -1.0;
+                w[e] = i < nk ? Heat::rounded(scaled[e]) : 0ull;
+                sum_w += w[e];
             }
             u64 sum;
-            const u64 incl = block_scan64(w[0] + w[1], s.scan, sum);
+            u64 front = block_scan64(sum_w, s.scan, sum) - sum_w;
             const u64 z_top = k > 0 ? sum : whole;
             target = static_cast<u64>(static_cast<double>(fmaxf(p, 0.f)) * static_cast<double>(z_top));
-            for (int i = tid; i < static_cast<int>(n); i += kThreads) s.weight[i] = 0;
+            for (int i = tid; i < count; i += kThreads) weight_of[i] = 0;
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const u64 front = e == 0 ? incl - w[0] - w[1] : incl - w[1];
-                if (place[e] >= 0 && (!(p < 1.0f) || front <= target) && scaled[e] >= bound) s.weight[place[e]] = w[e];
+            for (int e = 0; e < kEach; ++e) {
+                if (scaled[e] >= bound && (!(p < 1.0f) || front <= target))
+                    weight_of[0xffffffffu - static_cast<unsigned>(order[kEach * tid + e])] = w[e];
+                front += w[e];
             }
             __syncthreads();
             // cumulated in the order of indices
-            u64 z, c2[2];
+            u64 z;
+            sum_w = 0;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) c2[e] = 2 * tid + e < static_cast<int>(n) ? s.weight[2 * tid + e] : 0ull;
-            const u64 incl2 = block_scan64(c2[0] + c2[1], s.scan, z);
-            if (2 * tid < static_cast<int>(n)) s.weight[2 * tid] = incl2 - c2[1];
-            if (2 * tid + 1 < static_cast<int>(n)) s.weight[2 * tid + 1] = incl2;
+            for (int e = 0; e < kEach; ++e) {
+                const int i = kEach * tid + e;
+                w[e] = i < count ? weight_of[i] : 0ull;
+                sum_w += w[e];
+            }
+            front = block_scan64(sum_w, s.scan, z) - sum_w;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                front += w[e];
+                if (kEach * tid + e < count) weight_of[kEach * tid + e] = front;
+            }
             __syncthreads();
             for (int j = tid; j < draws; j += kThreads) {
                 const u64 goal = drawn_mass(uniform[draw0 + j], z);
-                int lo = 0, hi = static_cast<int>(n) - 1;
+                int lo = 0, hi = count - 1;
                 while (lo < hi) {
                     const int mid = (lo + hi) >> 1;
-                    if (s.weight[mid] > goal) hi = mid;
+                    if (weight_of[mid] > goal) hi = mid;
                     else lo = mid + 1;
                 }
-                out[draw0 + j] = s.all[lo].at;
-                if (prob) prob[draw0 + j] = static_cast<float>(heat.scaled(value_of(s.all[lo].key)) / static_cast<double>(z));
+                out[draw0 + j] = all_of[lo].at;
+                if (prob) prob[draw0 + j] = static_cast<float>(heat.scaled(value_of(all_of[lo].key)) / static_cast<double>(z));
             }
             return;
         }
@@ -842,10 +832,11 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
             }
         }
     }
-    auto kept_weight = [&](int i, float raw) -> u64 {
-        const float x = logit_of(raw);
-        const unsigned key = key_of(x);
-        return key > cut_key || (key == cut_key && i <= tie_cut) ? heat.weight(x) : 0ull;
+    // (as floats: key 0 is below all of them, and NaN, which has no weight, is never larger)
+    const bool cut_none = cut_key < key_of(-INFINITY);
+    const float cut_x = cut_none ? -INFINITY : value_of(cut_key);
+    auto kept_weight = [&](int i, float x) -> u64 {
+        return x > cut_x || (x == cut_x && i <= tie_cut) ? heat.weight(x) : 0ull;
     };
 
     // ---- masses: a lane's are those of a contiguous block of its warp's segment (an odd number of tokens: no two lanes
@@ -890,12 +881,13 @@ template <typename T>
 int launch_draw(const void* logits, long long stride, int rows, int V, const Settings& set, const float* uniform, int draws,
                 int* out, float* prob, cudaStream_t stream) {
     int ranks = 1;
-    while (ranks < 8 && V > ranks * 4096) ranks *= 2;
+    const auto bytes_of = [&](int n) { return static_cast<long long>(V) / n * static_cast<long long>(sizeof(T)); };
+    while (ranks < 8 && V > ranks * 4096 && !(rows * ranks >= 256 && bytes_of(ranks) <= 78 * 1024)) ranks *= 2;
     const int most = 192 * 1024;             // bytes of a slice beside the static shared memory
     const auto segment = [&](int n) { return ((V + n * kWarps - 1) / (n * kWarps) + 7) / 8 * 8; };
     while (ranks < kMaxCluster && static_cast<long long>(segment(ranks)) * kWarps * sizeof(T) > most) ranks *= 2;
     const int seg = segment(ranks);
-    const long long bytes = static_cast<long long>(seg) * kWarps * sizeof(T);
+    const long long bytes = std::max(static_cast<long long>(seg) * kWarps * static_cast<long long>(sizeof(T)), 24ll * kListed);
     if (bytes > most || V >= 1 << 20 || static_cast<long long>(rows) * ranks > 0x7fffffffll) return SOMI_ERR_UNSUPPORTED;
     allow_smem<draw_kernel<T>>(most);
     if (ranks > 8 && cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
