@@ -33,11 +33,11 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     __shared__ GroupScratch group_scratch;
     const Groups groups = hold_groups(b, group_scratch);      // [descriptor]
-    const Range range = find_range<kThreads>(b, groups, scratch);
+    __shared__ unsigned owned[kOwned];
+    const Range range = find_range<kThreads>(b, groups, scratch, owned);
     pdl_wait();
-    write_notes<kThreads>(b, groups, scratch, range.total, notes, header);
 
-    Walk walk(b, groups, range);
+    Walk walk(range);
     Piece p;
     while (walk.next(b, groups, p)) {
         const int rows = p.tokens * b.per;
@@ -152,7 +152,7 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
         for (int i = 0; i < 4; ++i) {
             const int row = ty * 4 + i;
             if (row >= rows) continue;
-            const size_t at = part_row(b, p.x.pos0 == 0x3fffffff, p.first, blockIdx.x, kRows, p.token0 + row / b.per,
+            const size_t at = part_row(b, p.x.pos0 == 0x3fffffff, p.first, blockIdx.x, p.token0 + row / b.per,
                                        p.kvh * b.per + row % b.per, row);
 #pragma unroll
             for (int c = 0; c < COLS; ++c)
@@ -160,6 +160,7 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
             if (tx == 0) parts.ml[at] = make_float2(m[i], l[i]);
         }
     }
+    write_notes<kThreads>(b, groups, owned, range.total, notes, header, tid);
 }
 
 constexpr int kMergeWarps = 4;
@@ -169,7 +170,7 @@ constexpr int kMergeWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const unsigned* __restrict__ header, Parts parts,
-                    int ctas, int block_rows, T* __restrict__ out) {
+                    int ctas, T* __restrict__ out) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31;
@@ -177,26 +178,26 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
     if (row >= static_cast<long long>(b.T) * b.nq) return;
     const int t = static_cast<int>(row / b.nq), h = static_cast<int>(row % b.nq), kvh = h / b.per;
     const unsigned total = header[0];
-    const Note note[2] = {notes[t], notes[b.T + t]};                 // prefix, own keys (the first may be unwritten)
+    const Note prefix = notes[t], own = notes[b.T + t];              // (the first may be unwritten)
     if (b.cu_q && (t < b.cu_q[0] || t >= b.cu_q[b.R])) return;       // a row of no request stays as it was
     if (total == 0) return;
     const Shares shares(total, ctas);
-    // the CTAs that had a part of the item, neighbours all
-    unsigned begin[2], first_cta[2], n_cta[2];
-    int place[2];
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        const Note& n = note[w];
-        place[w] = n.place & ((1 << 30) - 1);
-        begin[w] = n.begin + static_cast<unsigned>(kvh) * n.cost;
-        const unsigned end = begin[w] + n.cost;
+    // the CTAs that had a part of an item, neighbours all
+    struct Item { unsigned begin, first_cta, ctas; int place; };
+    auto item_of = [&](const Note& n, bool written) {
+        Item x;
+        x.place = n.place & ~kHasPrefix;
+        x.begin = n.begin + static_cast<unsigned>(kvh) * n.cost;
+        const unsigned end = x.begin + n.cost;
         // (the second half: what no note of a request's token looks like)
-        const bool there = (w == 1 || (note[1].place >> 30 & 1)) && n.units > 0 && n.cost == n.units + kOverhead && end <= total &&
-                           end >= begin[w] && place[w] >= 0 && (place[w] + 1) * b.per <= block_rows;
-        first_cta[w] = there ? shares.cta_of(begin[w]) : 0;
-        n_cta[w] = there ? shares.cta_of(end - 1) - first_cta[w] + 1 : 0;
-    }
-    const unsigned all = n_cta[0] + n_cta[1];
+        const bool there = written && n.units > 0 && n.cost == n.units + kOverhead && end <= total && end >= x.begin && x.place >= 0 &&
+                           (x.place + 1) * b.per <= b.block_rows;
+        x.first_cta = there ? shares.cta_of(x.begin) : 0u;
+        x.ctas = there ? shares.cta_of(end - 1) - x.first_cta + 1 : 0u;
+        return x;
+    };
+    const Item front = item_of(prefix, own.place & kHasPrefix), back = item_of(own, true);
+    const unsigned all = front.ctas + back.ctas;
     constexpr int COLS = 2;                          // of four columns a lane: head sizes to 256
     float m = -INFINITY, l = 0.f;
     F4 o[COLS];
@@ -207,11 +208,13 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
         size_t at = 0;
         float2 ml = make_float2(-INFINITY, 0.f);
         if (p < all) {
-            const int w = p < n_cta[0] ? 0 : 1;
-            const unsigned cta = first_cta[w] + (w ? p - n_cta[0] : p), c0 = shares.begin(cta), c1 = shares.begin(cta + 1);
-            const unsigned o0 = c0 > begin[w] ? c0 - begin[w] : 0, o1 = min(c1 - begin[w], static_cast<unsigned>(note[w].cost));
+            const bool first = p < front.ctas;
+            const unsigned begin = first ? front.begin : back.begin, cost = first ? prefix.cost : own.cost;
+            const unsigned cta = first ? front.first_cta + p : back.first_cta + p - front.ctas;
+            const unsigned c0 = shares.begin(cta), c1 = shares.begin(cta + 1);
+            const unsigned o0 = c0 > begin ? c0 - begin : 0, o1 = min(c1 - begin, cost);
             if (o1 > static_cast<unsigned>(kOverhead) && o1 > o0) {  // (else it had only the item's fixed cost)
-                at = part_row(b, w == 0, o0 == 0, cta, block_rows, t, h, place[w] * b.per + h % b.per);
+                at = part_row(b, first, o0 == 0, cta, t, h, (first ? front.place : back.place) * b.per + h % b.per);
                 ml = parts.ml[at];
             }
         }
@@ -279,68 +282,69 @@ int launch_shared(const Batch& b, const void* q, long long q_stride, const void*
 using namespace somi;
 using namespace somi::shp;
 
-// CTAs of a call (whichever kernel), and the rows of one CTA's continuation: what a caller needs for the workspace.
-static int shared_ctas(int per_sm) {
+// The kernels: 0 the one for any size, 1 the one on tensor cores, 2 that for few rows.  CTAs, and the rows of one CTA's continuation.
+SOMI_API int somi_shared_attention_ctas(int hd, int kernel) {
     int device = 0, sms = 0;
     cudaGetDevice(&device);
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) return 0;
-    return sms * per_sm;
+    return sms * (kernel == 2 ? 3 : kernel == 1 ? 1 : hd <= 64 ? 4 : hd <= 128 ? 2 : 1);
 }
-SOMI_API int somi_shared_attention_ctas(int hd, int tensor_cores) {
-    return shared_ctas(tensor_cores ? 1 : hd <= 64 ? 4 : hd <= 128 ? 2 : 1);
-}
-SOMI_API int somi_shared_attention_block_rows(int tensor_cores) {
-    return tensor_cores ? somi_shared_attention_tc_block_rows() : kRows;
+SOMI_API int somi_shared_attention_block_rows(int kernel) {
+    return kernel == 2 ? kFewRows : kernel == 1 ? somi_shared_attention_tc_block_rows() : kRows;
 }
 
 // Bytes of workspace: notes, the header, maxima and sums, outputs.
-static long long workspace_bytes(long long T, int nq, int hd, int ctas, int block_rows) {
-    const long long rows = 2 * T * nq + static_cast<long long>(ctas) * block_rows;
+static long long workspace_bytes(long long T, long long rows, int hd) {
     return 2 * T * static_cast<long long>(sizeof(Note)) + 32 + rows * 8 + rows * hd * 4;
 }
 
 // qkv [T, >= nq hd] (rows `q_stride` elements apart), keys and values [num_pages, nkv, page_size, hd], block_table
 // [R, bt_stride], cu_q [R + 1] or null (then T = R, one token per request), ctx_len [R], group_off [G + 1], prefix_len [G];
-// `out` [T, nq hd].  `tensor_cores`: by attention_shared_tcgen05.cu (where somi_shared_attention_tc_takes says so).
-// Refuses what it cannot take; the lengths are read on the device.
+// `out` [T, nq hd].  `kernel`: see above (1 and 2 where somi_shared_attention_tc_takes says so, 2 for at most 16 rows a
+// key/value head).  Refuses what it cannot take; the lengths are read on the device.
 SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_stride, const void* keys, const void* values,
                                    const int* block_table, int bt_stride, const int* cu_q, const int* ctx_len,
                                    const int* prefix_len, const int* group_off, int T, int R, int G, int nq, int nkv, int hd,
-                                   int page_size, int num_pages, float scale, int tensor_cores, void* workspace,
-                                   long long bytes, int ctas, void* out, cudaStream_t stream) {
+                                   int page_size, int num_pages, float scale, int kernel, void* workspace, long long bytes,
+                                   int ctas, void* out, cudaStream_t stream) {
     if (T <= 0 || R <= 0) return 0;
-    if (nkv <= 0 || nq <= 0 || nq % nkv || (!tensor_cores && nq / nkv > kRows) || hd % 16 || hd < 16 || hd > 256 || G < 0 || bt_stride <= 0 ||
-        page_size <= 0 || num_pages <= 0 || ctas <= 0 || static_cast<long long>(R) + G > kMaxEntries ||
+    if (nkv <= 0 || nq <= 0 || nq % nkv || (!kernel && nq / nkv > kRows) || hd % 16 || hd < 16 || hd > 256 || G < 0 || bt_stride <= 0 ||
+        page_size <= 0 || num_pages <= 0 || kernel < 0 || kernel > 2 || ctas <= 0 || static_cast<long long>(R) + G > kMaxEntries ||
         static_cast<long long>(R) + G > static_cast<long long>(ctas) * kOwned || (!cu_q && T != R))
         return SOMI_ERR_UNSUPPORTED;
+    const int per = nq / nkv;
+    if (kernel && (dtype != SOMI_BF16 || !somi_shared_attention_tc_takes(nq, nkv, hd, page_size))) return SOMI_ERR_UNSUPPORTED;
+    if (kernel == 2 && static_cast<long long>(T) * per > kFewRows) return SOMI_ERR_UNSUPPORTED;
     const long long span = static_cast<long long>(bt_stride) * page_size;
-    if (tensor_cores && (dtype != SOMI_BF16 || !somi_shared_attention_tc_takes(nq, nkv, hd, page_size))) return SOMI_ERR_UNSUPPORTED;
-    const int block_rows = somi_shared_attention_block_rows(tensor_cores);
-    const int item_tokens = (tensor_cores ? block_rows / 2 : kRows) / (nq / nkv);
+    const int block_rows = somi_shared_attention_block_rows(kernel);
+    const int item_tokens = (kernel == 1 ? block_rows / 2 : block_rows) / per;
     const long long items = (R + static_cast<long long>(G) + 2 * (T / item_tokens + 1ll)) * nkv;
-    if (span > 0x3fff0000ll || items * (span / kKeys + 3) > 0x7fffffffll || static_cast<long long>(T) * nq / kMergeWarps >= 0x7fffffffll)
+    if (span > 0x3fff0000ll || items * (span / kKeys + 3) > 0x7fffffffll || static_cast<long long>(T) * nq / kMergeWarps >= 0x7fffffffll ||
+        static_cast<long long>(num_pages) * nkv * page_size > 0x7fffffffll)
         return SOMI_ERR_UNSUPPORTED;
+    const long long rows = 2ll * T * nq + static_cast<long long>(ctas) * block_rows;
     if (reinterpret_cast<uintptr_t>(workspace) % 32) return SOMI_ERR_UNSUPPORTED;
-    if (bytes < workspace_bytes(T, nq, hd, ctas, block_rows)) return SOMI_ERR_SCRATCH_TOO_SMALL;
-    Batch b{cu_q, ctx_len, prefix_len, group_off, block_table, bt_stride, R, G, T, nq, nkv, nq / nkv, page_size, num_pages,
-            item_tokens, item_tokens, kKeys, kKeys, kKeys};
+    if (bytes < workspace_bytes(T, rows, hd)) return SOMI_ERR_SCRATCH_TOO_SMALL;
+    const Batch b{cu_q, ctx_len, prefix_len, group_off, block_table, bt_stride, R, G, T, nq, nkv, per, page_size, num_pages,
+                  item_tokens, item_tokens, kKeys, kKeys, kKeys, block_rows};
     char* at = static_cast<char*>(workspace);
     Note* notes = reinterpret_cast<Note*>(at);
     unsigned* header = reinterpret_cast<unsigned*>(at + 2ll * T * sizeof(Note));
-    const long long rows = 2ll * T * nq + static_cast<long long>(ctas) * block_rows;
     Parts parts;
     parts.o = reinterpret_cast<float*>(header + 8);      // (on a boundary of 32 bytes, as the workspace is)
     parts.ml = reinterpret_cast<float2*>(parts.o + rows * hd);
     const auto launch = [&](auto kind) {
         using E = decltype(kind);
-        int rc = tensor_cores ? shared_attention_tc(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
-                 : hd <= 64   ? launch_shared<E, 64>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
-                 : hd <= 128  ? launch_shared<E, 128>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
-                              : launch_shared<E, 256>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream);
+        const int rc =
+            kernel == 2 ? shared_attention_rows(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
+            : kernel == 1 ? shared_attention_tc(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
+            : hd <= 64    ? launch_shared<E, 64>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
+            : hd <= 128   ? launch_shared<E, 128>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
+                          : launch_shared<E, 256>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream);
         if (rc) return rc;
         const long long out_rows = static_cast<long long>(T) * nq;
         return launch_pdl(shared_merge_kernel<E>, dim3(static_cast<unsigned>((out_rows + kMergeWarps - 1) / kMergeWarps)),
-                          dim3(kMergeWarps * 32), 0, stream, b, hd, notes, header, parts, ctas, block_rows, static_cast<E*>(out));
+                          dim3(kMergeWarps * 32), 0, stream, b, hd, notes, header, parts, ctas, static_cast<E*>(out));
     };
     return dtype == SOMI_F32 ? launch(float{}) : dtype == SOMI_BF16 ? launch(__nv_bfloat16{}) : SOMI_ERR_UNSUPPORTED;
 }

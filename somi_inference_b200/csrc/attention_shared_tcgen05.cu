@@ -108,6 +108,7 @@ struct Tail {
     float a_top[kTile];
     PieceNote ring[kPieces];
     GroupScratch groups;
+    unsigned owned[kOwned];
     uint32_t tmem_base;
     int failed, softmax_failed[2];
 };
@@ -171,12 +172,11 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     const Groups groups = hold_groups(b, tail.groups);                // [descriptor]
-    const Range range = find_range<kTcThreads>(b, groups, scratch);   // [descriptor]
+    const Range range = find_range<kTcThreads>(b, groups, scratch, tail.owned);   // [descriptor]
     t5::fence_before();
     __syncthreads();
     t5::fence_after();
     pdl_wait();
-    write_notes<kTcThreads>(b, groups, scratch, range.total, notes, header);
     fence_proxy_async();                                              // (the scratch lies where copies will arrive)
     __syncthreads();
     const uint32_t tmem_s = tmem_base_s, tmem_o = tmem_base_s + 2 * kTile;
@@ -191,7 +191,7 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         if (warp == 11) {
             // ---- the pieces, one after the other
-            Walk walk(b, groups, range);
+            Walk walk(range);
             Piece p;
             int last_wide = -1;
             bool more = true, ok = true;
@@ -229,6 +229,8 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                 }
                 __syncwarp();
             }
+            // (what the merge wants to know: while the others work on the last pieces)
+            write_notes<32>(b, groups, tail.owned, range.total, notes, header, lane);
         } else if (warp == 8 || warp == 10) {
             // ---- producers of keys and of values: lane 0 keeps the barriers, a lane per page copies it
             const int which = warp == 8 ? 0 : 1;
@@ -250,7 +252,7 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                     const int kb = p.key0 + t * kTile;
                     const int pos = kb + lane * b.page_size;
                     int page = -1;
-                    if (lane < pages_per_tile && pos < p.key_hi && pos + b.page_size > p.key_lo) page = table[pos / b.page_size];
+                    if (lane < pages_per_tile && pos < p.key_hi && pos + b.page_size > p.key_lo) page = ld_step(table + pos / b.page_size);
                     const bool mine = static_cast<unsigned>(page) < static_cast<unsigned>(b.num_pages);
                     const int n_pages = __popc(__ballot_sync(0xffffffffu, mine));
                     int st, round;
@@ -539,7 +541,7 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
 
             const int head = p.kvh * b.per + row % b.per, token = p.token0 + my_token;
             const bool mine = row < live;
-            const size_t at = part_row(b, p.prefix != 0, p.first != 0, blockIdx.x, kTcBlockRows, token, head,
+            const size_t at = part_row(b, p.prefix != 0, p.first != 0, blockIdx.x, token, head,
                                        my_token * b.per + row % b.per);
             if (wide) {
                 if (mine) parts.ml[at] = make_float2(m, l);

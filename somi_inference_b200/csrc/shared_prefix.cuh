@@ -28,6 +28,7 @@ namespace shp {
 constexpr int kOverhead = 1;        // cost of an item beside its units
 constexpr int kMaxEntries = 8192;   // groups and requests of a call
 constexpr int kOwned = 64;          // entries whose tokens one CTA notes for the merge, at most
+constexpr int kFewRows = 16;        // query rows of an entry that attention_shared_rows.cu takes
 
 struct Batch {
     const int *cu_q;                // [R + 1], or null: one token per request
@@ -36,6 +37,7 @@ struct Batch {
     int item_tokens;                // tokens of a tile, at most
     int wide_tokens;                // entries of more tokens than this have units of `unit_wide` keys
     int unit_narrow, unit_wide, align;
+    int block_rows;                 // rows of a CTA's continuation
 };
 
 // The groups' borders and prefixes as a block reads them: its own copies where they are few.
@@ -45,8 +47,9 @@ struct Groups {
 
 // What joins the parts: per token, for the prefix and for its own keys, where the item of its first
 // key/value head begins in the order of costs, what an item costs, how many units it has, and the
-// token's place in the tile.
+// token's place in the tile (with a flag).
 struct Note { unsigned begin; int cost, units, place; };
+constexpr int kHasPrefix = 1 << 30;
 
 struct Entry {
     int first, tokens;              // rows of the batch
@@ -121,13 +124,14 @@ struct Range {
     unsigned begin, end;            // this CTA's
     int entry;                      // the entry that holds `begin`
     unsigned entry_base;            // where that entry begins
+    Entry at;                       // that entry
 };
 
 struct RangeScratch {
     unsigned warp_sum[32];
     int entry;
     unsigned entry_base;
-    unsigned owned[kOwned];
+    Entry at;                       // that entry
 };
 
 constexpr int kGroupsHeld = 31;     // groups that a block copies
@@ -145,18 +149,18 @@ __device__ __forceinline__ Groups hold_groups(const Batch& b, GroupScratch& s) {
     return Groups{s.off, s.prefix};
 }
 
-// All threads of the block.  Writes the notes of the entries that this CTA owns and header[0] = all costs (CTA 0).
+// All threads of the block.  owned[k]: where entry blockIdx.x + k gridDim.x begins, whose tokens this CTA notes.
 template <int THREADS>
-__device__ __forceinline__ Range find_range(const Batch& b, const Groups& gs, RangeScratch& s) {
+__device__ __forceinline__ Range find_range(const Batch& b, const Groups& gs, RangeScratch& s, unsigned* owned) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int E = b.G + b.R, each = (E + THREADS - 1) / THREADS;
     const int e0 = tid * each, e1 = min(e0 + each, E);
-    unsigned mine = 0, first_cost = 0;
+    unsigned mine = 0;
+    Entry first_entry;
     for (int e = e0; e < e1; ++e) {
         const Entry x = entry_of(b, gs, e);
-        const unsigned c = static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
-        if (e == e0) first_cost = c;
-        mine += c;
+        if (e == e0) first_entry = x;
+        mine += static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
     }
     unsigned incl = mine;
 #pragma unroll
@@ -182,41 +186,41 @@ __device__ __forceinline__ Range find_range(const Batch& b, const Groups& gs, Ra
     const bool holds = r.begin >= before && r.begin < before + mine;
     unsigned at = before;
     for (int e = e0; e < e1; ++e) {
-        unsigned c = first_cost;
-        if (each > 1) {
-            const Entry x = entry_of(b, gs, e);
-            c = static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
-        }
+        const Entry x = e == e0 ? first_entry : entry_of(b, gs, e);
+        const unsigned c = static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
         if (holds && r.begin >= at && r.begin < at + c) {
             s.entry = e;
             s.entry_base = at;
+            s.at = x;
         }
-        if (e % gridDim.x == blockIdx.x) s.owned[e / gridDim.x] = at;
+        if (e % gridDim.x == blockIdx.x) owned[e / gridDim.x] = at;
         at += c;
     }
     __syncthreads();
     r.entry = s.entry;
     r.entry_base = s.entry_base;
+    r.at = s.at;
     return r;
 }
 
-// The notes of this CTA's entries.  `notes`: [2][T], prefixes first.  After the wait for the kernels in front.
+// The notes of this CTA's entries.  `notes`: [2][T], prefixes first; header[0]: all costs.  After the wait for the kernels
+// in front.
 template <int THREADS>
-__device__ __forceinline__ void write_notes(const Batch& b, const Groups& gs, const RangeScratch& s, unsigned total, Note* notes,
-                                            unsigned* header) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) header[0] = total;
+__device__ __forceinline__ void write_notes(const Batch& b, const Groups& gs, const unsigned* owned, unsigned total, Note* notes,
+                                            unsigned* header, int thread) {
+    if (blockIdx.x == 0 && thread == 0) header[0] = total;
     for (int e = blockIdx.x, k = 0; e < b.G + b.R; e += gridDim.x, ++k) {
         const Entry x = entry_of(b, gs, e);
-        if (e < b.G && x.tiles == 0) continue;      // the requests' own notes say that there is no prefix
+        if (e < b.G && x.tiles == 0) continue;      // (the requests' own notes say whether there is a prefix)
         Note* to = notes + (e < b.G ? 0 : b.T) + x.first;
-        for (int t = threadIdx.x; t < x.tokens; t += THREADS) {
+        for (int t = thread; t < x.tokens; t += THREADS) {
             Note n;
             const int j = t / b.item_tokens;
-            n.begin = s.owned[k] + static_cast<unsigned>(j) * x.cost() * b.nkv;
+            n.begin = owned[k] + static_cast<unsigned>(j) * x.cost() * b.nkv;
             n.cost = x.cost();
             n.units = x.units;
             n.place = t - j * b.item_tokens;
-            if (e >= b.G && x.key_lo > 0) n.place |= 1 << 30;       // there is a prefix in front
+            if (e >= b.G && x.key_lo > 0) n.place |= kHasPrefix;
             if (x.tiles == 0) n.units = 0;
             to[t] = n;
         }
@@ -238,9 +242,7 @@ struct Walk {
     int e;
     unsigned base;
     Entry x;
-    __device__ __forceinline__ Walk(const Batch& b, const Groups& gs, const Range& r) : at(r.begin), end(r.end), e(r.entry), base(r.entry_base) {
-        if (at < end) x = entry_of(b, gs, e);
-    }
+    __device__ __forceinline__ Walk(const Range& r) : at(r.begin), end(r.end), e(r.entry), base(r.entry_base), x(r.at) {}
     __device__ __forceinline__ bool next(const Batch& b, const Groups& gs, Piece& p) {
         while (at < end) {
             unsigned whole = static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
@@ -270,19 +272,20 @@ struct Walk {
     }
 };
 
-// Where the rows of a piece go.  Rows of first pieces: (token, head); of continuations: the CTA's block.
+// Where the rows of a piece go.  Rows of first pieces: (token, head), of prefixes and of own keys; of continuations: the CTA's block.
 struct Parts {
-    float* o;                       // [(2 T nq + N block_rows), hd]
-    float2* ml;                     // [2 T nq + N block_rows]
+    float* o;                       // [rows, hd]
+    float2* ml;                     // [rows]
 };
-__device__ __forceinline__ size_t part_row(const Batch& b, bool prefix, bool first, int cta, int block_rows,
-                                           int token, int head, int row_in_item) {
-    const size_t dense = static_cast<size_t>(b.T) * b.nq;
-    if (first) return (prefix ? 0 : dense) + static_cast<size_t>(token) * b.nq + head;
-    return 2 * dense + static_cast<size_t>(cta) * block_rows + row_in_item;
+__device__ __forceinline__ size_t part_row(const Batch& b, bool prefix, bool first, int cta, int token, int head, int row_in_item) {
+    if (first) return ((prefix ? 0 : static_cast<size_t>(b.T)) + token) * b.nq + head;
+    return 2 * static_cast<size_t>(b.T) * b.nq + static_cast<size_t>(cta) * b.block_rows + row_in_item;
 }
 
-// The tensor-core kernel (attention_shared_tcgen05.cu): sets its own sizes of tiles in `b`.
+// The kernels on tensor cores, for calls of few rows (attention_shared_rows.cu) and for any (attention_shared_tcgen05.cu):
+// they set their own sizes of tiles in `b`.
+int shared_attention_rows(Batch b, const void* q, long long q_stride, const void* keys, const void* values, int hd, float scale,
+                          Note* notes, unsigned* header, Parts parts, int ctas, cudaStream_t stream);
 int shared_attention_tc(Batch b, const void* q, long long q_stride, const void* keys, const void* values, int hd, float scale,
                         Note* notes, unsigned* header, Parts parts, int ctas, cudaStream_t stream);
 

@@ -113,7 +113,7 @@ class CudaOps:
         self.use_tma_prefill = True
         self._gemm_maps: dict = {}
         self.use_shared_tc = True
-        # type, heads, sizes -> whether on tensor cores, CTAs and rows of a block of attention over shared prefixes
+        # type, heads, sizes, few tokens -> the kernel of attention over shared prefixes, its CTAs, rows of a CTA's block
         self._shared_plans: dict = {}
         self._shared_attention = self.lib.somi_shared_attention
         p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
@@ -686,48 +686,58 @@ class CudaOps:
         numbers of requests, groups and tokens).  bfloat16 or float32, head sizes in multiples of 16 up to
         256, at most 64 query heads a key/value head and 8,192 requests and groups.
         """
-        if not (qkv.dim() == 2 and qkv.stride(1) == 1 and tuple(out.shape) == (qkv.shape[0], nq * hd)
-                and qkv.shape[1] >= nq * hd and out.dtype == kcache.dtype == vcache.dtype == qkv.dtype):
-            raise KernelError("queries are [T, width >= heads * head size] with contiguous rows, the output [T, heads * head "
-                              "size], both of the cache's dtype")
-        ints = (block_table, ctx_len, prefix_len, group_off) + (() if cu_q is None else (cu_q,))
-        _check(out, kcache, vcache, *ints)
-        if not qkv.is_cuda or any(t.device != out.device for t in (qkv, kcache, vcache, *ints)) \
-                or out.device.index != self._device_index or torch.cuda.current_device() != self._device_index:
+        # (few Python operations: a call of few rows takes 8 us on the device)
+        ints = (block_table, ctx_len, prefix_len, group_off) if cu_q is None else (block_table, ctx_len, prefix_len, group_off, cu_q)
+        dtype, device, T, R, G = qkv.dtype, self._device_index, qkv.shape[0], ctx_len.numel(), prefix_len.numel()
+        for t in (out, kcache, vcache):
+            if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+                raise KernelError("shared_prefix_attention: output and cache are contiguous, of the queries' dtype and on the "
+                                  "kernel table's device")
+        for t in ints:
+            if t.dtype is not torch.int32 or t.get_device() != device or not t.is_contiguous():
+                raise KernelError("shared_prefix_attention: block_table, ctx_len, prefix_len, group_off and cu_q are contiguous, "
+                                  "int32 and on the kernel table's device")
+        if qkv.get_device() != device or torch.cuda.current_device() != device:
             raise KernelError("shared_prefix_attention: all tensors on the kernel table's device, which is the current one")
-        T, R, G = qkv.shape[0], ctx_len.numel(), prefix_len.numel()
-        if any(t.dtype != torch.int32 for t in ints) or kcache.shape != vcache.shape or kcache.dim() != 4 \
-                or tuple(kcache.shape[1::2]) != (nkv, hd) or block_table.dim() != 2 or block_table.shape[0] != R \
-                or group_off.numel() != G + 1 or (cu_q is not None and cu_q.numel() != R + 1) or (cu_q is None and T != R):
-            raise KernelError("a shared batch has int32 block_table [R, width], ctx_len [R], prefix_len [G], group_off [G + 1] "
-                              "and cu_q [R + 1] (without it T = R tokens), and caches [pages, kv heads, page size, head size]")
+        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < nq * hd or out.shape != (T, nq * hd):
+            raise KernelError("queries are [T, width >= heads * head size] with contiguous rows, the output [T, heads * head size]")
+        if kcache.dim() != 4:
+            raise KernelError("caches are [pages, kv heads, page size, head size]")
+        pages, kv_heads, page_size, width = kcache.shape
+        if vcache.shape != kcache.shape or kv_heads != nkv or width != hd or block_table.dim() != 2 or block_table.shape[0] != R \
+                or group_off.numel() != G + 1 or (T != R if cu_q is None else cu_q.numel() != R + 1):
+            raise KernelError("a shared batch has block_table [R, width], ctx_len [R], prefix_len [G], group_off [G + 1] and cu_q "
+                              "[R + 1] (without it T = R tokens), and caches [pages, kv heads, page size, head size]")
         self.check_attention_geometry(nq, nkv, hd)
-        pages, page_size = kcache.shape[0], kcache.shape[2]
-        if (qkv.stride(0) * qkv.element_size()) % 16 or qkv.data_ptr() % 16 or out.data_ptr() % 16 \
-                or kcache.data_ptr() % 16 or vcache.data_ptr() % 16:
+        at = (qkv.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr())
+        row = qkv.stride(0)
+        if (at[0] | at[1] | at[2] | at[3] | row * dtype.itemsize) % 16:
             raise KernelError("query rows, outputs and caches begin on 16-byte boundaries")
         if T == 0 or R == 0:
             return
         code = _code(qkv)
-        key = (code, nq, nkv, hd, page_size, self.use_shared_tc)
+        key = (code, nq, nkv, hd, page_size, self.use_shared_tc, min(T, 17))
         plan = self._shared_plans.get(key)
         if plan is None:
-            tc = int(code == _BF16 and self.use_shared_tc
-                     and bool(self.lib.somi_shared_attention_tc_takes(nq, nkv, hd, page_size)))
-            plan = self._shared_plans[key] = (tc, int(self.lib.somi_shared_attention_ctas(hd, tc)),
-                                              int(self.lib.somi_shared_attention_block_rows(tc)))
-        tc, ctas, block_rows = plan
+            # 0 the kernel for any size, 1 the one on tensor cores, 2 that for up to 16 rows a key/value head
+            kernel = 0
+            if code == _BF16 and self.use_shared_tc and self.lib.somi_shared_attention_tc_takes(nq, nkv, hd, page_size):
+                kernel = 2 if T * (nq // nkv) <= 16 else 1
+            plan = self._shared_plans[key] = (kernel, int(self.lib.somi_shared_attention_ctas(hd, kernel)),
+                                              int(self.lib.somi_shared_attention_block_rows(kernel)))
+        kernel, ctas, block_rows = plan
         rows = 2 * T * nq + ctas * block_rows
-        work = torch.empty(32 * T + 32 + rows * (8 + 4 * hd), dtype=torch.uint8, device=qkv.device)
+        nbytes = 32 * T + 32 + rows * (8 + 4 * hd)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=qkv.device)
         rc = self._shared_attention(
-            qkv.data_ptr(), code, qkv.stride(0), kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(),
-            block_table.shape[1], None if cu_q is None else cu_q.data_ptr(), ctx_len.data_ptr(), prefix_len.data_ptr(),
-            group_off.data_ptr(), T, R, G, nq, nkv, hd, page_size, pages, scale, tc, work.data_ptr(), work.numel(), ctas,
-            out.data_ptr(), self._stream())
+            at[0], code, row, at[1], at[2], block_table.data_ptr(), block_table.shape[1], None if cu_q is None else cu_q.data_ptr(),
+            ctx_len.data_ptr(), prefix_len.data_ptr(), group_off.data_ptr(), T, R, G, nq, nkv, hd, page_size, pages, scale, kernel,
+            work.data_ptr(), nbytes, ctas, at[3], self._stream())
         self._done(rc, "shared_prefix_attention")
         self.launches += 1
         if trace.active():
-            trace.note("attention_shared_tcgen05" if tc else "attention_shared", 2 * T * nq * hd * qkv.element_size(), detail="with merge; without keys and values")
+            trace.note(("attention_shared", "attention_shared_tcgen05", "attention_shared_rows")[kernel],
+                       2 * T * nq * hd * qkv.element_size(), detail="with merge; without keys and values")
 
     def two_map_attention(self, qkv, kcache, vcache, batch, group, nq, nkv, d, vd, scale, window, keep,
                           factor: float, eps: float, gain: float, gate, out, storage=None) -> None:
@@ -2226,36 +2236,39 @@ class CudaOps:
         `penalty` [rows] with `hist_off` int32 [rows + 1] and `hist_tok` int32 (a row's history, every token
         once): repetition penalty in front of everything else (float32 logits), as in `sample`.
         """
-        history = () if penalty is None else (penalty, hist_off, hist_tok)
-        if any(t is None for t in history):
-            raise KernelError("a repetition penalty comes with hist_off and hist_tok")
-        given = (uniform, temperature, top_k, top_p, min_p, out, *(() if prob is None else (prob,)), *history)
-        _check(*given)
-        if not (logits.is_cuda and logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
-            raise KernelError("logits are [rows, vocabulary] with contiguous rows on the device")
+        # (few Python operations: a call takes 12 us on the device)
+        device = self._device_index
+        if logits.dim() != 2 or logits.get_device() != device or torch.cuda.current_device() != device:
+            raise KernelError("logits are [rows, vocabulary] on the kernel table's device, which is the current one")
         rows, V = logits.shape
-        if any(t.device != logits.device for t in given) or logits.device.index != self._device_index \
-                or torch.cuda.current_device() != self._device_index:
-            raise KernelError("draw_tokens: all tensors on the kernel table's device, which is the current one")
-        if uniform.dim() not in (1, 2) or uniform.shape[0] != rows or out.shape != uniform.shape \
-                or (prob is not None and prob.shape != uniform.shape) \
-                or any(t.numel() != rows for t in (temperature, top_k, top_p, min_p)) \
-                or (penalty is not None and (penalty.numel() != rows or hist_off.numel() != rows + 1)):
+        if logits.stride(1) != 1 and V != 1:
+            raise KernelError("logits have contiguous rows")
+        floats, ints, history = (uniform, temperature, top_p, min_p), (top_k, out), penalty is not None
+        if prob is not None:
+            floats += (prob,)
+        if history:
+            if hist_off is None or hist_tok is None:
+                raise KernelError("a repetition penalty comes with hist_off and hist_tok")
+            if logits.dtype is not torch.float32 or penalty.numel() != rows or hist_off.numel() != rows + 1:
+                raise KernelError("a repetition penalty takes float32 logits, penalty [rows] and hist_off [rows + 1]")
+            floats, ints = floats + (penalty,), ints + (hist_off, hist_tok)
+        for group, kind in ((floats, torch.float32), (ints, torch.int32)):
+            for t in group:
+                if t.dtype is not kind or t.get_device() != device or not t.is_contiguous():
+                    raise KernelError("draw_tokens: contiguous float32 numbers, settings and probabilities, int32 top_k, tokens and "
+                                      "history, all on the kernel table's device")
+        shape = uniform.shape
+        if len(shape) not in (1, 2) or shape[0] != rows or out.shape != shape or (prob is not None and prob.shape != shape) \
+                or temperature.numel() != rows or top_k.numel() != rows or top_p.numel() != rows or min_p.numel() != rows:
             raise KernelError("draw_tokens takes uniform, out and prob of one shape, [rows] or [rows, draws], and settings [rows]")
-        if any(t.dtype != torch.float32 for t in (uniform, temperature, top_p, min_p, *(() if prob is None else (prob,)),
-                                                  *history[:1])) \
-                or any(t.dtype != torch.int32 for t in (top_k, out, *history[1:])):
-            raise KernelError("draw_tokens: float32 numbers and settings, int32 top_k, tokens and history")
-        if penalty is not None and logits.dtype != torch.float32:
-            raise KernelError("a repetition penalty takes float32 logits")
-        draws = uniform.shape[1] if uniform.dim() == 2 else 1
+        draws = shape[1] if len(shape) == 2 else 1
         code = _code(logits)
         if rows == 0 or draws == 0:
             return
         rc = self._draw(logits.data_ptr(), code, logits.stride(0), rows, V, uniform.data_ptr(), draws, temperature.data_ptr(),
-                        top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(), *(t.data_ptr() for t in history or ()),
-                        *(() if history else (None, None, None)), out.data_ptr(), None if prob is None else prob.data_ptr(),
-                        self._stream())
+                        top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(), penalty.data_ptr() if history else None,
+                        hist_off.data_ptr() if history else None, hist_tok.data_ptr() if history else None, out.data_ptr(),
+                        None if prob is None else prob.data_ptr(), self._stream())
         self._done(rc, "draw_tokens")
         if trace.active():
             trace.note("draw", rows * V * logits.element_size(), detail=f"{draws} draws" if draws > 1 else "")

@@ -6,16 +6,23 @@ import pytest
 import torch
 
 from somi_inference_b200.ops import KernelError, cuda
-from tests.test_kernel_table import OnDevice
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that the host side takes for one of device 0's."""
+    is_cuda = True
+
+    def get_device(self):
+        return 0
 
 
 @pytest.fixture
 def ops(monkeypatch):
     table = cuda.CudaOps.__new__(cuda.CudaOps)
-    table.launches, table._device_index, table.calls = 0, None, []
+    table.launches, table._device_index, table.calls = 0, 0, []
     table._draw = lambda *a: table.calls.append(a) or 0
     table._stream = lambda: ctypes.c_void_p(0)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     return table
 
 

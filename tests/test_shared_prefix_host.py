@@ -6,7 +6,14 @@ import pytest
 import torch
 
 from somi_inference_b200.ops import KernelError, cuda
-from tests.test_kernel_table import OnDevice
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that the host side takes for one of device 0's."""
+    is_cuda = True
+
+    def get_device(self):
+        return 0
 
 
 def on_device(t):
@@ -17,14 +24,14 @@ def on_device(t):
 def ops(monkeypatch):
     """A kernel table over CPU tensors whose launcher notes its calls."""
     table = cuda.CudaOps.__new__(cuda.CudaOps)
-    table.launches, table._device_index, table.calls = 0, None, []
+    table.launches, table._device_index, table.calls = 0, 0, []
     table._shared_plans, table.use_shared_tc = {}, True
     table.lib = type("Library", (), {})()
-    table.lib.somi_shared_attention_ctas = lambda hd, tc: 148
-    table.lib.somi_shared_attention_block_rows = lambda tc: 64
+    table.lib.somi_shared_attention_ctas = lambda hd, kernel: 148
+    table.lib.somi_shared_attention_block_rows = lambda kernel: 64
     table._shared_attention = lambda *a: table.calls.append(a) or 0
     table._stream = lambda: ctypes.c_void_p(0)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     return table
 
 
