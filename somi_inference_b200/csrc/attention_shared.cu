@@ -190,7 +190,7 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
         x.begin = n.begin + static_cast<unsigned>(kvh) * n.cost;
         const unsigned end = x.begin + n.cost;
         // (the second half: what no note of a request's token looks like)
-        const bool there = written && n.units > 0 && n.cost == n.units + kOverhead && end <= total && end >= x.begin && x.place >= 0 &&
+        const bool there = written && n.units > 0 && n.cost > n.units && end <= total && end >= x.begin && x.place >= 0 &&
                            (x.place + 1) * b.per <= b.block_rows;
         x.first_cta = there ? shares.cta_of(x.begin) : 0u;
         x.ctas = there ? shares.cta_of(end - 1) - x.first_cta + 1 : 0u;
@@ -210,10 +210,11 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
         if (p < all) {
             const bool first = p < front.ctas;
             const unsigned begin = first ? front.begin : back.begin, cost = first ? prefix.cost : own.cost;
+            const unsigned over = cost - static_cast<unsigned>(first ? prefix.units : own.units);
             const unsigned cta = first ? front.first_cta + p : back.first_cta + p - front.ctas;
             const unsigned c0 = shares.begin(cta), c1 = shares.begin(cta + 1);
             const unsigned o0 = c0 > begin ? c0 - begin : 0, o1 = min(c1 - begin, cost);
-            if (o1 > static_cast<unsigned>(kOverhead) && o1 > o0) {  // (else it had only the item's fixed cost)
+            if (o1 > over && o1 > o0) {  // (else it had only the item's fixed cost)
                 at = part_row(b, first, o0 == 0, cta, t, h, (first ? front.place : back.place) * b.per + h % b.per);
                 ml = parts.ml[at];
             }
@@ -326,7 +327,7 @@ SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_strid
     if (reinterpret_cast<uintptr_t>(workspace) % 32) return SOMI_ERR_UNSUPPORTED;
     if (bytes < workspace_bytes(T, rows, hd)) return SOMI_ERR_SCRATCH_TOO_SMALL;
     const Batch b{cu_q, ctx_len, prefix_len, group_off, block_table, bt_stride, R, G, T, nq, nkv, per, page_size, num_pages,
-                  item_tokens, item_tokens, kKeys, kKeys, kKeys, block_rows};
+                  item_tokens, item_tokens, kKeys, kKeys, kKeys, 1, block_rows};
     char* at = static_cast<char*>(workspace);
     Note* notes = reinterpret_cast<Note*>(at);
     unsigned* header = reinterpret_cast<unsigned*>(at + 2ll * T * sizeof(Note));

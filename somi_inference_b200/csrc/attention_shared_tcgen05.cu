@@ -33,6 +33,9 @@ namespace shp {
 
 constexpr int kTcThreads = 384, kTile = 128;          // rows of a warp group; keys of a tile
 constexpr int kTcBlockRows = 2 * kTile;
+// An item of more than 128 rows gathers 256 rows of queries and writes 256 of outputs, and often comes between pieces of the other way:
+// with a cost of 3 beside its units, where one of few rows has 1, 24 portions of 1 to 47 tokens behind 20,000 positions take 157 us (1: 278).
+constexpr int kOverWide = 3;
 constexpr int kPieces = 4;                            // of the ring of pieces
 constexpr int kHalf = kTile * 128;                    // bytes of a [128][64] swizzled block
 __host__ __device__ constexpr int k_stages(int hd) { return hd == 128 ? 2 : 4; }
@@ -629,6 +632,7 @@ int shared_attention_tc(Batch b, const void* q, long long q_stride, const void* 
     b.item_tokens = 2 * b.wide_tokens;
     b.align = b.unit_wide = kTile;
     b.unit_narrow = 2 * kTile;
+    b.over_wide = kOverWide;
     return hd == 64 ? launch_tc<64>(k_map, v_map, b, q, q_stride, scale, notes, header, parts, ctas, stream)
                     : launch_tc<128>(k_map, v_map, b, q, q_stride, scale, notes, header, parts, ctas, stream);
 }

@@ -6,8 +6,8 @@
 // group's prefix, or the tokens of one request over its own positions behind the prefix.  Entries
 // 0 .. G-1 are the groups, G .. G+R-1 the requests.  An entry's tokens are cut into tiles of
 // `item_tokens`; a tile for one key/value head is an *item*, its rows are the tile's tokens times the
-// query heads of that head, and its keys are cut into *units*.  An item costs its units and `kOverhead`
-// more, and the costs of all items, one behind the other, are shared out evenly over the CTAs in
+// query heads of that head, and its keys are cut into *units*.  An item costs its units and one unit
+// more, or `over_wide` (queries to be gathered, rows to be written), and the costs of all items, one behind the other, are shared out evenly over the CTAs in
 // contiguous ranges (U / N costs each, the first U % N of them one more).  So any mixture of long and
 // short entries fills the chip evenly, whatever the lengths are, and the host has to know none of them
 // (a captured graph runs with new lengths).  Every CTA adds the entries' costs up by itself (a few loads and one scan over the
@@ -25,7 +25,6 @@
 namespace somi {
 namespace shp {
 
-constexpr int kOverhead = 1;        // cost of an item beside its units
 constexpr int kMaxEntries = 8192;   // groups and requests of a call
 constexpr int kOwned = 64;          // entries whose tokens one CTA notes for the merge, at most
 constexpr int kFewRows = 16;        // query rows of an entry that attention_shared_rows.cu takes
@@ -37,6 +36,7 @@ struct Batch {
     int item_tokens;                // tokens of a tile, at most
     int wide_tokens;                // entries of more tokens than this have units of `unit_wide` keys
     int unit_narrow, unit_wide, align;
+    int over_wide;                  // what their items cost beside their units (others: 1)
     int block_rows;                 // rows of a CTA's continuation
 };
 
@@ -57,7 +57,8 @@ struct Entry {
     int key_lo, key_hi;             // keys [key_lo, key_hi)
     int pos0;                       // position of the first token: token i sees keys up to pos0 + i
     int tiles, unit, units;         // tiles of tokens, keys of a unit, units of an item
-    __device__ __forceinline__ int cost() const { return units + kOverhead; }
+    int over;                       // what an item costs beside its units
+    __device__ __forceinline__ int cost() const { return units + over; }
     __device__ __forceinline__ int base(const Batch& b) const { return key_lo / b.align * b.align; }
 };
 
@@ -100,7 +101,9 @@ __device__ __forceinline__ Entry entry_of(const Batch& b, const Groups& gs, int 
         x.key_hi = min(ctx + x.tokens, span);
         x.pos0 = ctx;
     }
-    x.unit = x.tokens > b.wide_tokens ? b.unit_wide : b.unit_narrow;
+    const bool wide = x.tokens > b.wide_tokens;
+    x.unit = wide ? b.unit_wide : b.unit_narrow;
+    x.over = wide ? b.over_wide : 1;
     const bool some = x.tokens > 0 && x.key_hi > x.key_lo;
     x.tiles = some ? (x.tokens + b.item_tokens - 1) / b.item_tokens : 0;
     x.units = some ? (x.key_hi - x.base(b) + x.unit - 1) / x.unit : 0;
@@ -256,8 +259,9 @@ struct Walk {
             const unsigned item = (at - base) / cost, o = (at - base) - item * cost;
             const unsigned stop = min(end - at + o, cost);
             at += stop - o;
-            p.unit0 = o > kOverhead ? o - kOverhead : 0;
-            p.unit1 = stop > kOverhead ? stop - kOverhead : 0;
+            const unsigned over = x.over;
+            p.unit0 = o > over ? o - over : 0;
+            p.unit1 = stop > over ? stop - over : 0;
             p.tile = item / b.nkv;
             p.kvh = item % b.nkv;
             p.first = o == 0;
