@@ -16,7 +16,7 @@ constexpr int kRows = 64, kKeys = 64, kThreads = 256;
 
 // HD: the head size rounded up to 64, 128 or 256; d: the head size (a multiple of 16)
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1)
 shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stride, const T* __restrict__ keys,
                         const T* __restrict__ values, int d, float scale_log2e, Note* __restrict__ notes,
                         unsigned* __restrict__ header, Parts parts) {
@@ -42,13 +42,12 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
     while (walk.next(b, groups, p)) {
         const int rows = p.tokens * b.per;
         __syncthreads();
-        for (int i = tid; i < kRows * (HD / 4); i += kThreads) {
-            const int row = i / (HD / 4), c = (i % (HD / 4)) * 4;
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) {
+            const int i = tid + n * kThreads, row = i / (HD / 4), c = (i % (HD / 4)) * 4, t = row / b.per;
             F4 v{{0.f, 0.f, 0.f, 0.f}};
-            if (row < rows && c < d) {
-                const int token = p.token0 + row / b.per, head = p.kvh * b.per + row % b.per;
-                v = load4(q + token * q_stride + static_cast<size_t>(head) * d + c);
-            }
+            if (row < rows && c < d)
+                v = load4(q + (p.token0 + t) * q_stride + static_cast<size_t>(p.kvh * b.per + row - t * b.per) * d + c);
             store4(Qs + row * LD + c, v);
         }
         float m[4], l[4], o[4][COLS];
@@ -68,24 +67,41 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
         }
         const int kb0 = p.x.base(b);
         const int* table = b.block_table + static_cast<size_t>(p.x.table) * b.bt_stride;
-        // one tile of keys or values; what lies outside the piece's keys, or on no page, becomes zeros
-        auto load_tile = [&](const T* __restrict__ from, int k0) {
-            for (int i = tid; i < kKeys * (HD / 4); i += kThreads) {
-                const int key = i / (HD / 4), c = (i % (HD / 4)) * 4, pos = k0 + key;
-                F4 v{{0.f, 0.f, 0.f, 0.f}};
+        // A tile of keys or values on its way to shared memory: loaded into registers while the products of the tile in front
+        // are computed.  What lies outside the piece's keys, or on no page, becomes zeros.
+        F4 tile[HD / 16];
+        auto fetch = [&](const T* __restrict__ from, int k0) {
+            const T* at[HD / 16];
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) {
+                const int i = tid + n * kThreads, key = i / (HD / 4), c = (i % (HD / 4)) * 4, pos = k0 + key;
+                at[n] = nullptr;
                 if (c < d && pos >= p.x.key_lo && pos < p.x.key_hi) {
                     const int page = table[pos / b.page_size];
                     if (static_cast<unsigned>(page) < static_cast<unsigned>(b.num_pages))
-                        v = load4(from + ((static_cast<size_t>(page) * b.nkv + p.kvh) * b.page_size + pos % b.page_size) * d + c);
+                        at[n] = from + ((static_cast<size_t>(page) * b.nkv + p.kvh) * b.page_size + pos % b.page_size) * d + c;
                 }
-                store4(KV + key * LD + c, v);
+            }
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) {
+                tile[n] = F4{{0.f, 0.f, 0.f, 0.f}};
+                if (at[n]) tile[n] = load4(at[n]);
             }
         };
+        auto put = [&]() {
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) {
+                const int i = tid + n * kThreads;
+                store4(KV + (i / (HD / 4)) * LD + (i % (HD / 4)) * 4, tile[n]);
+            }
+        };
+        fetch(keys, kb0 + p.unit0 * p.x.unit);
         for (int u = p.unit0; u < p.unit1; ++u) {
             const int k0 = kb0 + u * p.x.unit;
             __syncthreads();
-            load_tile(keys, k0);
+            put();
             __syncthreads();
+            fetch(values, k0);
             float s[4][4] = {};
             for (int c = 0; c < HD; c += 4) {
                 F4 a[4], k[4];
@@ -129,8 +145,9 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
                 for (int c = 0; c < COLS; ++c) o[i][c] *= keep;
             }
             __syncthreads();                         // all threads have read the keys
-            load_tile(values, k0);
+            put();
             __syncthreads();
+            if (u + 1 < p.unit1) fetch(keys, k0 + p.x.unit);
             // (a value that a row does not see stays out of its sum even if it is infinite)
             const bool all_seen = k0 + kKeys - 1 <= p.x.pos0;
             for (int j = 0; j < kKeys; j += 4) {
