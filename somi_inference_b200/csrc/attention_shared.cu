@@ -180,18 +180,21 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
     write_notes<kThreads>(b, groups, owned, range.total, notes, header, tid);
 }
 
-constexpr int kMergeWarps = 4;
+constexpr int kFewRowsOut = 4 * 148;     // four blocks an SM
 
-// A warp per (token, head).  A lane finds out where a part lies and loads its maximum and sum, for up to 32 parts at once;
-// then all lanes add the parts' outputs up, several loads in flight.
-template <typename T>
-__global__ void __launch_bounds__(kMergeWarps * 32)
+// SPLIT warps per (token, head), a block of WARPS.  A lane finds out where a part lies and loads its maximum and sum, for
+// up to 32 parts at once; then all lanes add the parts' outputs up, several loads in flight.  The parts go round the row's
+// warps, whose sums are joined in shared memory.
+template <typename T, int WARPS, int SPLIT>
+__global__ void __launch_bounds__(WARPS * 32)
 shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const unsigned* __restrict__ header, Parts parts,
                     int ctas, T* __restrict__ out) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31;
-    const long long row = static_cast<long long>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
+    const int warp = (threadIdx.x >> 5) % SPLIT;
+    const long long row = static_cast<long long>(blockIdx.x) * (WARPS / SPLIT) + (threadIdx.x >> 5) / SPLIT;
+    static_assert(SPLIT == 1 || SPLIT == WARPS, "the returns below are the whole block's where it joins its warps");
     if (row >= static_cast<long long>(b.T) * b.nq) return;
     const int t = static_cast<int>(row / b.nq), h = static_cast<int>(row % b.nq), kvh = h / b.per;
     const unsigned total = header[0];
@@ -220,8 +223,8 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
     F4 o[COLS];
 #pragma unroll
     for (int c = 0; c < COLS; ++c) o[c] = F4{{0.f, 0.f, 0.f, 0.f}};
-    for (unsigned p0 = 0; p0 < all; p0 += 32) {
-        const unsigned p = p0 + lane;
+    for (unsigned p0 = 0; p0 < all; p0 += 32 * SPLIT) {
+        const unsigned p = p0 + lane * SPLIT + warp;
         size_t at = 0;
         float2 ml = make_float2(-INFINITY, 0.f);
         if (p < all) {
@@ -271,6 +274,33 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
                     for (int e = 0; e < 4; ++e) o[c].v[e] = fmaf(v[k][c].v[e], w[k], o[c].v[e]);
             left = rest;
         }
+    }
+    if constexpr (SPLIT > 1) {
+        __shared__ float2 state[SPLIT];
+        __shared__ __align__(16) float rows[SPLIT][256];
+        if (lane == 0) state[warp] = make_float2(m, l);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+            if ((c * 32 + lane) * 4 < d) store4(&rows[warp][(c * 32 + lane) * 4], o[c]);
+        __syncthreads();
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < SPLIT; ++w) top = fmaxf(top, state[w].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float f[SPLIT];
+#pragma unroll
+        for (int w = 0; w < SPLIT; ++w) {
+            f[w] = exp2f(state[w].x - ref);
+            sum = fmaf(state[w].y, f[w], sum);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        for (int col = threadIdx.x; col < d; col += WARPS * 32) {
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < SPLIT; ++w) v = fmaf(rows[w][col], f[w], v);
+            out[row * d + col] = from_float<T>(v * inv);
+        }
+        return;
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
@@ -337,7 +367,7 @@ SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_strid
     const int block_rows = somi_shared_attention_block_rows(kernel);
     const int item_tokens = (kernel == 1 ? block_rows / 2 : block_rows) / per;
     const long long items = (R + static_cast<long long>(G) + 2 * (T / item_tokens + 1ll)) * nkv;
-    if (span > 0x3fff0000ll || items * (span / kKeys + 3) > 0x7fffffffll || static_cast<long long>(T) * nq / kMergeWarps >= 0x7fffffffll ||
+    if (span > 0x3fff0000ll || items * (span / kKeys + 3) > 0x7fffffffll || static_cast<long long>(T) * nq >= 0x1fffffffcll ||
         static_cast<long long>(num_pages) * nkv * page_size > 0x7fffffffll)
         return SOMI_ERR_UNSUPPORTED;
     const long long rows = 2ll * T * nq + static_cast<long long>(ctas) * block_rows;
@@ -361,8 +391,14 @@ SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_strid
                           : launch_shared<E, 256>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream);
         if (rc) return rc;
         const long long out_rows = static_cast<long long>(T) * nq;
-        return launch_pdl(shared_merge_kernel<E>, dim3(static_cast<unsigned>((out_rows + kMergeWarps - 1) / kMergeWarps)),
-                          dim3(kMergeWarps * 32), 0, stream, b, hd, notes, header, parts, ctas, static_cast<E*>(out));
+        // Few rows have their keys in many CTAs.  One warp a row against eight: 2 requests behind 8,192 positions 32.4 us and
+        // 12.5 (14 heads of 64), 8 behind 2,048 14.5 and 13.5 (28 of 128), 32 behind 4,096 19.4 and 16.4 (448 rows), but 896 rows
+        // 22.8 and 25.1.  Up to 8 steps of 64 keys there is nothing to divide (2 behind 176: 7.0 and 7.3).
+        if (out_rows <= kFewRowsOut && span > 512)
+            return launch_pdl(shared_merge_kernel<E, 8, 8>, dim3(static_cast<unsigned>(out_rows)), dim3(256), 0, stream, b, hd, notes,
+                              header, parts, ctas, static_cast<E*>(out));
+        return launch_pdl(shared_merge_kernel<E, 4, 1>, dim3(static_cast<unsigned>((out_rows + 3) / 4)), dim3(128), 0, stream, b, hd,
+                          notes, header, parts, ctas, static_cast<E*>(out));
     };
     return dtype == SOMI_F32 ? launch(float{}) : dtype == SOMI_BF16 ? launch(__nv_bfloat16{}) : SOMI_ERR_UNSUPPORTED;
 }
