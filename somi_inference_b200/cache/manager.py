@@ -24,6 +24,9 @@ What this manager does differently:
 * Every request also gets a *state slot*: an index into per-run tensors of fixed
   size `[num_slots, ...]` for mixers whose memory does not grow with length.
   The slot's tensors are zeroed when the request registers.
+* A request can be *forked* off another one: it shares the other's first whole pages instead of having
+  them computed and kept again (`fork`).  Shared pages are only read; they go back to the pool with their last holder.
+  Requests that share are a family, which the batch builder finds by `family`.
 * `reserve` is all-or-nothing across groups: either every group has the pages
   for the new tokens or `OutOfPages` is raised and nothing changed.
 """
@@ -122,6 +125,8 @@ class CacheManager:
         self._slot_of: dict[object, int] = {}
         self._len: dict[object, int] = {}
         self._reserved: dict[object, int] = {}
+        self._family: dict[object, tuple[int, int]] = {}     # request -> (family, positions it shares with it)
+        self._families = 0
         self.groups: list[_Group] = []
         self._views: list[CacheView | None] = [None] * len(needs_per_run)
 
@@ -185,6 +190,41 @@ class CacheManager:
             for t in view.state.values():
                 t[slot].zero_()
         return slot
+
+    def fork(self, req: object, of: object, n_tokens: int) -> int:
+        """Admit a request whose first `n_tokens` positions (a multiple of the page size) are those of `of`, as
+        far as they are cached: it starts with that length.  Returns the slot."""
+        if of not in self._slot_of:
+            raise ValueError(f"request {of!r} is not registered")
+        if n_tokens <= 0 or n_tokens % self.page_size or n_tokens > self._len[of]:
+            raise ValueError(f"a fork shares whole pages ({self.page_size} positions) of what is cached of {of!r} "
+                             f"({self._len[of]}), not {n_tokens} positions")
+        if any(g.needs.window is not None for g in self.groups):
+            raise ValueError("pages of a window are given back one by one: requests with windows cannot be forked")
+        if any(v is not None and v.state for v in self._views):
+            raise ValueError("states of fixed size are not kept for earlier positions: requests with states cannot be forked")
+        slot, source = self.register(req), self._slot_of[of]
+        n = n_tokens // self.page_size
+        for g in self.groups:
+            g.pool.share([int(p) for p in g.tables[source, :n]])
+            g.tables[slot, :n] = g.tables[source, :n]
+            g.num_blocks[slot] = n
+        self._len[req] = n_tokens
+        if of not in self._family:
+            self._families += 1
+            self._family[of] = (self._families, n_tokens)
+        family, shared = self._family[of]
+        self._family[req] = (family, min(shared, n_tokens))
+        return slot
+
+    @property
+    def any_family(self) -> bool:
+        return bool(self._family)
+
+    def family(self, req: object) -> tuple[int, int]:
+        """(family, first positions that the request has in common with all of it); (0, 0): shares nothing.
+        A fork of a fork is counted with what its whole family shares, whatever more it shares with the one."""
+        return self._family.get(req, (0, 0))
 
     def slot(self, req: object) -> int:
         return self._slot_of[req]
@@ -266,6 +306,7 @@ class CacheManager:
         slot = self._slot_of.pop(req)
         del self._len[req]
         del self._reserved[req]
+        self._family.pop(req, None)
         for g in self.groups:
             g.pool.give_back(g.held(slot))
             g.tables[slot, :int(g.num_blocks[slot])] = FREED
@@ -285,16 +326,20 @@ class CacheManager:
         return self.groups[group].held(self._slot_of[req])
 
     def check_consistency(self) -> None:
-        """Every page is either free or held by exactly one live request (used by tests)."""
+        """Every page is either free or held by as many live requests as the pool counts, more than one only
+        where requests were forked (used by tests)."""
         for gi, g in enumerate(self.groups):
-            seen: set[int] = set()
+            seen: dict[int, int] = {}
             for req in self._slot_of:
                 for p in self.held_pages(req, gi):
-                    if p in seen:
+                    seen[p] = seen.get(p, 0) + 1
+                    if seen[p] > 1 and req not in self._family:
                         raise AssertionError(f"page {p} of group {gi} is held twice")
                     if not g.pool.is_held(p):
                         raise AssertionError(f"page {p} of group {gi} is in a table but free")
-                    seen.add(p)
+            for p, n in seen.items():
+                if n != g.pool.holders(p):
+                    raise AssertionError(f"page {p} of group {gi} is held by {n} requests, the pool counts {g.pool.holders(p)}")
             if len(seen) != g.pool.num_held:
                 raise AssertionError(f"group {gi}: {g.pool.num_held} pages held by the pool, "
                                      f"{len(seen)} found in tables (a page was lost)")

@@ -41,6 +41,16 @@ class GroupBatch:
 
 
 @dataclass
+class SharedPrefixes:
+    """Neighbouring requests of the batch that share their first positions (forks, `CacheManager.fork`)."""
+
+    prefix_len: torch.Tensor        # int32 [G] positions that group g's requests share (0: none)
+    group_off: torch.Tensor         # int32 [G + 1] group g is requests [group_off[g], group_off[g + 1])
+    # bits of the number of positions that need not be read again: sum of prefix_len * (members - 1)
+    saved_bits: int
+
+
+@dataclass
 class HostBatch:
     """Host copies of the small arrays, for parts that plan on the host."""
 
@@ -73,6 +83,7 @@ class StepBatch:
     # the sizes that fix every offset in the buffer, then the multi-token requests and their tokens:
     # two steps with equal keys launch the same kernels with the same arguments
     layout_key: tuple = field(default_factory=tuple)
+    shared: SharedPrefixes | None = None    # None: no two requests of the step share anything
 
 
 _NO_TILES = np.zeros((0, 3), dtype=np.int64)
@@ -111,6 +122,29 @@ class BatchBuilder:
         self._dev = torch.empty(capacity, dtype=torch.int32, device=self.device)
         self._capacity = capacity
         self.generation = getattr(self, "generation", 0) + 1    # device addresses changed
+
+    def _shared_runs(self, requests) -> tuple[list[int], list[int], int] | None:
+        """(borders of the runs of neighbours that share, what each shares, bits of what that saves), or None."""
+        if not self.cache.any_family:
+            return None
+        off, shared, last, saved = [0], [], None, 0
+        for j, r in enumerate(requests):
+            family, n = self.cache.family(r)
+            if j and (family != last or not family):
+                off.append(j)
+            if off[-1] == j:
+                shared.append(n)
+            else:
+                shared[-1] = min(shared[-1], n)
+            last = family
+        off.append(len(requests))
+        for g, n in enumerate(shared):
+            members = off[g + 1] - off[g]
+            shared[g] = n if members > 1 else 0
+            saved += shared[g] * (members - 1)
+        if not saved:
+            return None
+        return off, shared, saved.bit_length()
 
     @property
     def h2d_bytes_last(self) -> int:
@@ -210,6 +244,10 @@ class BatchBuilder:
         arrays += [tiles_np[bm].reshape(-1) for bm in self.q_tile_sizes]
         for gi in range(len(tables)):
             arrays += [tables[gi].reshape(-1), slot_maps[gi]]
+        runs = self._shared_runs([entries[i].request for i in order])
+        if runs:
+            sizes += [len(runs[0]), len(runs[1])]
+            arrays += runs[:2]
         offsets, total = self._upload(sizes, arrays)
 
         def dv(k: int) -> torch.Tensor:
@@ -220,6 +258,7 @@ class BatchBuilder:
         g0 = n_fixed + len(self.q_tile_sizes)
         groups = [GroupBatch(dv(g0 + 2 * gi).view(R, widths[gi]), dv(g0 + 2 * gi + 1), widths[gi])
                   for gi in range(len(tables))]
+        at = len(sizes)
         batch = StepBatch(
             num_tokens=T, num_requests=R, num_prefill_requests=n_prefill,
             num_prefill_tokens=n_prefill_tokens, max_q_len=int(q_lens.max()),
@@ -228,7 +267,8 @@ class BatchBuilder:
             state_slot=dv(5), logit_rows=dv(6), tiles=tiles, groups=groups,
             host=HostBatch(cu_q=cu_q, ctx_len=ctx, state_slot=slots,
                            requests=[entries[i].request for i in order]),
-            layout_key=tuple(sizes) + (n_prefill, n_prefill_tokens),
+            layout_key=tuple(sizes) + (n_prefill, n_prefill_tokens) + (runs[2:] if runs else ()),
+            shared=SharedPrefixes(dv(at - 1), dv(at - 2), runs[2]) if runs else None,
         )
         return batch, order
 
@@ -281,8 +321,12 @@ class BatchBuilder:
         arrays += [() for _ in self.q_tile_sizes]
         for gi in range(len(tables)):
             arrays += [tables[gi].reshape(-1), slot_maps[gi]]
+        runs = self._shared_runs(reqs)
+        if runs:
+            sizes += [len(runs[0]), len(runs[1])]
+            arrays += runs[:2]
         offsets, total = self._upload(sizes, arrays)
-        key = tuple(sizes)
+        key = tuple(sizes) + (bool(runs),)
         views = self._decode_views.get(key)
         if views is None or views[0] is not self._dev:
             # the device views depend on the sizes only: made once per layout
@@ -294,11 +338,12 @@ class BatchBuilder:
             g0 = n_fixed + len(self.q_tile_sizes)
             groups = [GroupBatch(dv(g0 + 2 * gi).view(R, widths[gi]), dv(g0 + 2 * gi + 1), widths[gi])
                       for gi in range(len(tables))]
-            views = (self._dev, [dv(k) for k in range(7)], tiles, groups)
+            shared = (dv(len(sizes) - 1), dv(len(sizes) - 2)) if runs else None
+            views = (self._dev, [dv(k) for k in range(7)], tiles, groups, shared)
             if len(self._decode_views) > 256:
                 self._decode_views.clear()
             self._decode_views[key] = views
-        _, fixed, tiles, groups = views
+        _, fixed, tiles, groups, shared = views
         batch = StepBatch(
             num_tokens=R, num_requests=R, num_prefill_requests=0, num_prefill_tokens=0,
             max_q_len=1, max_kv_len=max_kv, token_ids=fixed[0], positions=fixed[1],
@@ -306,7 +351,8 @@ class BatchBuilder:
             logit_rows=fixed[6], tiles=tiles, groups=groups,
             host=HostBatch(cu_q=np.arange(R + 1, dtype=np.int64), ctx_len=pos_np,
                            state_slot=slots_np, requests=reqs),
-            layout_key=tuple(sizes) + (0, 0))
+            layout_key=tuple(sizes) + (0, 0) + (runs[2:] if runs else ()),
+            shared=SharedPrefixes(*shared, runs[2]) if runs else None)
         return batch, list(range(R))
 
     def _current_stream(self):

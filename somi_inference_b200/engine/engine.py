@@ -278,6 +278,20 @@ class Engine:
         self.token_patch_bytes = 0
         return self._run(batch, keep)
 
+    def fork(self, request: object, of: object, tokens: int | None = None) -> int:
+        """Start `request` with the first `tokens` positions of `of` (all that are cached without them), in whole
+        pages: their keys and values are kept once, and steps in which such requests stand beside each other
+        attend to them once for all.  Returns how many positions `request` has now (0: less than a page is
+        shared, and nothing was registered); its next tokens continue from there.  Models with windows or
+        states refuse."""
+        cached = self.cache.length(of)
+        if tokens is not None and not 0 <= tokens <= cached:
+            raise ValueError(f"{tokens} positions of {of!r} are wanted, {cached} are cached")
+        shared = (cached if tokens is None else tokens) // self.page_size * self.page_size
+        if shared:
+            self.cache.fork(request, of, shared)
+        return shared
+
     def end(self, request: object) -> None:
         """The request is finished: everything it holds goes back to the pools."""
         self.cache.release(request)

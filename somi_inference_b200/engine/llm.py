@@ -284,12 +284,12 @@ class LLM:
     def generate(self, prompt: str | Sequence[int], *, max_new_tokens: int,
                  temperature: float = 1.0, top_k: int = -1, top_p: float = 1.0,
                  repetition_penalty: float = 1.0, seed: int | None = None,
-                 ignore_eos: bool = False) -> str | list[int]:
+                 ignore_eos: bool = False, min_p: float = 0.0) -> str | list[int]:
         """Generate for one prompt; return only what is new (text for text, ids for ids)."""
         is_text = isinstance(prompt, str)
         tokens = self._tok().encode(prompt, add_special_tokens=False) if is_text else list(prompt)
         sp = SamplingParams(temperature=temperature, top_k=top_k, top_p=top_p,
-                            repetition_penalty=repetition_penalty, seed=seed)
+                            repetition_penalty=repetition_penalty, seed=seed, min_p=min_p)
         req = self.make_request(tokens, max_new_tokens=max_new_tokens, sampling_params=sp,
                                 ignore_eos=ignore_eos)
         finished = self.run([(0, req)])

@@ -49,6 +49,7 @@ def parse_args(argv: list[str] | None = None) -> argparse.Namespace:
     p.add_argument("--temperature", type=float, default=1.0)
     p.add_argument("--top-k", type=int, default=-1)
     p.add_argument("--top-p", type=float, default=1.0)
+    p.add_argument("--min-p", type=float, default=0.0)
     p.add_argument("--repetition-penalty", type=float, default=1.0)
     p.add_argument("--chunk-size", type=int, default=512, help="Largest prompt portion per step.")
     p.add_argument("--max-num-batched-tokens", type=int, default=2048)
@@ -115,7 +116,7 @@ def main(argv: list[str] | None = None, *, ops=None, device=None) -> int:
         llm = LLM(args.model_name, num_blocks=args.num_blocks, block_size=args.block_size,
                   dtype=dtype, ops=ops, device=device, **common)
     kw = dict(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
-              repetition_penalty=args.repetition_penalty)
+              repetition_penalty=args.repetition_penalty, min_p=args.min_p)
     results = []
     if args.prompt is not None:
         text = llm.generate(args.prompt, max_new_tokens=args.max_new_tokens, seed=args.seed, **kw)

@@ -113,6 +113,7 @@ class CudaOps:
         self.use_tma_prefill = True
         self._gemm_maps: dict = {}
         self.use_shared_tc = True
+        self.use_shared_prefix = True
         # type, heads, sizes, few tokens -> the kernel of attention over shared prefixes, its CTAs, rows of a CTA's block
         self._shared_plans: dict = {}
         self._shared_attention = self.lib.somi_shared_attention
@@ -420,6 +421,13 @@ class CudaOps:
             assert turn.dtype == torch.float32 and tuple(turn.shape) == (out.shape[0], vd // 2, 2)
             if gate is not None or vd % 2:
                 raise KernelError("turned outputs come in pairs and without a gate")
+        shared = getattr(batch, "shared", None)
+        if shared is not None and self.shared_prefix_pays(shared.saved_bits, batch, nq, nkv, hd, qkv, page_size) and vd == hd and not (
+                win or chunk or cap or sinks is not None or turn is not None or gate is not None):
+            self.shared_prefix_attention(qkv, kcache, vcache, group.block_table, batch.ctx_len, shared.prefix_len,
+                                         shared.group_off, nq, nkv, hd, scale, out,
+                                         cu_q=batch.cu_q if batch.num_prefill_requests else None)
+            return
         prefill_turned = decode_turned = False      # whether the rows' kernel turned them
         n_decode = batch.num_requests - batch.num_prefill_requests
         # what the tensor-core kernels compute; they fetch query rows in 16-byte pieces
@@ -738,6 +746,32 @@ class CudaOps:
         if trace.active():
             trace.note(("attention_shared", "attention_shared_tcgen05", "attention_shared_rows")[kernel],
                        2 * T * nq * hd * qkv.element_size(), detail="with merge; without keys and values")
+
+    # What a step must save, in elements of keys of one run that it does not read again, to attend to shared prefixes
+    # once for all (times two: the host knows the saved positions by the length of their number), both ways measured:
+    # single tokens of bfloat16 at 28 heads of 128 over 4, 8 behind 2,048 (2^22 saved) 9.7 us and 13.8, 16 behind 2,048
+    # (2^23) 15.0 and 17.2, 8 behind 8,192 (2^24) 25.8 and 17.8, 64 behind 2,048 (2^25) 44.8 and 25.3; what every request
+    # has read once lies in L2, and a step takes the longer way of parts, products of whole tiles and a merge.
+    SHARED_PREFIX_VALUES = 1 << 25
+    # Short portions fill tiles of their own badly: 4 portions of 16 behind 512 (2^19) 16.6 us and 16.6, 2 behind 2,048
+    # (2^20) 40.9 and 19.1, 64 of 2 behind 64 (2^20) 72.5 and 19.2.  Longer ones gain only behind much longer prefixes:
+    # of 64, 16 behind 176 33.8 and 48.6, 8 behind 1,024 40.3 and 38.4, 16 behind 4,096 229.7 and 99.2; of 128, 16 behind
+    # 4,096 241 and 179; of 200 285 and 283.
+    SHARED_PREFIX_VALUES_PORTIONS = 1 << 20
+
+    def shared_prefix_pays(self, saved_bits: int, batch, nq: int, nkv: int, hd: int, qkv, page_size: int) -> bool:
+        """Whether a step of bfloat16 goes to `shared_prefix_attention`: where the positions that it does not read again
+        (a number of `saved_bits` bits) are worth more than its longer way."""
+        if not self.use_shared_prefix or qkv.dtype != torch.bfloat16 or qkv.shape[1] % 8 or batch.num_requests > 4096:
+            return False
+        portions, values = batch.num_prefill_requests, nkv * hd << saved_bits
+        if portions == 0:
+            pays = values >= self.SHARED_PREFIX_VALUES
+        else:
+            mean = batch.num_prefill_tokens / portions
+            pays = values >= self.SHARED_PREFIX_VALUES_PORTIONS and (
+                mean <= 32 or (mean <= 128 and 1 << saved_bits >= 32 * batch.num_tokens))
+        return pays and bool(self.lib.somi_shared_attention_tc_takes(nq, nkv, hd, page_size))
 
     def two_map_attention(self, qkv, kcache, vcache, batch, group, nq, nkv, d, vd, scale, window, keep,
                           factor: float, eps: float, gain: float, gate, out, storage=None) -> None:

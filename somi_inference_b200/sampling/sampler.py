@@ -3,7 +3,9 @@
 Same interface idea as the reference's `Sampler.sample(logits, params, token_histories)`
 (somi_inference/core/sampler.py:31-55), but the whole pipeline (repetition
 penalty, temperature, top-k, top-p, argmax or draw) is one kernel launch for
-all rows, and each row carries (seed, counter) for its random number.
+all rows, and each row carries (seed, counter) for its random number.  Rows with `min_p`, and draws
+from numbers that the caller brings (`draw`), go to the kernel that cuts exactly k tokens and makes any number of draws
+a row (`CudaOps.draw_tokens`).
 """
 
 from __future__ import annotations
@@ -45,7 +47,42 @@ class Sampler:
                 self._greedy[rows] = cached
             self.h2d_bytes_last = 0
             return self._launch(logits, rows, *cached)
-        return self._launch(logits, rows, *self._pack(params, counters, seeds, histories))
+        out = self._launch(logits, rows, *self._pack(params, counters, seeds, histories))
+        cut = [i for i, p in enumerate(params) if p.min_p > 0.0 and p.temperature > 0.0]
+        if cut:
+            # their rows by themselves, so that the other rows' tokens do not depend on them; the numbers are the ones that the
+            # rows would have drawn above
+            moved = self.h2d_bytes_last
+            number = torch.tensor([self.ops.uniform(int(seeds[i]) % (1 << 64), int(counters[i]) % (1 << 32)) for i in cut],
+                                  dtype=torch.float32)
+            all_rows = len(cut) == rows
+            at = None if all_rows else torch.tensor(cut, device=self.device)
+            tokens, _ = self.draw(logits if all_rows else logits[at], [params[i] for i in cut], number.to(self.device),
+                                  None if histories is None else [histories[i] for i in cut], probabilities=False)
+            if all_rows:
+                out = tokens
+            else:
+                out[at] = tokens
+            self.h2d_bytes_last += moved + 12 * len(cut)
+        return out
+
+    def draw(self, logits: torch.Tensor, params: Sequence[SamplingParams], uniforms: torch.Tensor,
+             histories: Sequence[Sequence[int]] | None = None, probabilities: bool = True):
+        """Tokens by numbers that the caller brings: logits [rows, vocab], `uniforms` float32 [rows], or [rows, n] for n
+        draws of every row (the first tokens of n continuations of one prompt, say), in [0, 1), on the
+        device.  Returns (int32 tokens, float32 probabilities that they were drawn with, or None), shaped as `uniforms`."""
+        rows = logits.shape[0]
+        if not (len(params) == rows == uniforms.shape[0]):
+            raise ValueError("one SamplingParams and one row of numbers per logits row is needed")
+        temperature, top_k, top_p, penalty, _, _, hist_off, hist_tok = self._pack(params, [0] * rows, [0] * rows, histories)
+        min_p = torch.tensor([p.min_p for p in params], dtype=torch.float32).to(self.device, non_blocking=True)
+        self.h2d_bytes_last += 4 * rows
+        out = torch.empty(uniforms.shape, dtype=torch.int32, device=self.device)
+        prob = torch.empty_like(uniforms) if probabilities else None
+        penalised = any(p.repetition_penalty != 1.0 for p in params)
+        self.ops.draw_tokens(logits, uniforms, temperature, top_k, top_p, min_p, out, prob=prob,
+                             **(dict(penalty=penalty, hist_off=hist_off, hist_tok=hist_tok) if penalised else {}))
+        return out, prob
 
     def _pack(self, params, counters, seeds, histories):
         rows = len(params)

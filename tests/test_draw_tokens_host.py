@@ -92,3 +92,15 @@ def test_what_the_launcher_refuses_is_an_error(ops):
     ops._draw = lambda *a: cuda.ERR_UNSUPPORTED
     with pytest.raises(KernelError, match="not supported"):
         ops.draw_tokens(**arguments())
+
+
+@pytest.mark.parametrize("value", [-0.1, 1.5, float("nan")])
+def test_min_p_has_a_range(value):
+    from somi_inference_b200 import SamplingParams
+    with pytest.raises(ValueError):
+        SamplingParams(min_p=value)
+
+
+def test_the_command_takes_min_p():
+    from somi_inference_b200.entrypoints.generate import parse_args
+    assert parse_args(["--model-name", "m", "--prompt", "p", "--min-p", "0.2"]).min_p == 0.2
