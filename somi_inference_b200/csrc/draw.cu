@@ -60,12 +60,9 @@ struct Shared {
         struct {
             union {
                 Token list[kListed];         // this CTA's survivors (likewise)
-                struct {                     // in the first CTA, where it cuts top-p's bin:
-                    u64 bin_order[kBinListed];       // the tokens by value,
-                    Token bin_all[kBinListed];       // and in the order of indices
-                };
+                u64 bin_order[kBinListed];   // in the first CTA, where it cuts top-p's bin: its tokens by value and index
             };
-            Token bin_list[kBinListed];      // this CTA's tokens of top-p's bin (likewise)
+            Token bin_list[kBinListed];      // this CTA's tokens of top-p's bin, in any order (read by the others)
         };
     };
     u64 scan[kWarps];
@@ -76,6 +73,7 @@ struct Shared {
     unsigned key[kWarps], at[kWarps];
     u64 cross_above, cross_mass;
     int cross_bin, tie_cut;
+    unsigned bin_count;                      // of bin_list; more than it holds: some are missing
     unsigned cut_key;
     unsigned lo, hi;
     unsigned long long loaded;               // mbarrier of the bulk copy
@@ -121,7 +119,7 @@ struct Heat {
         const double p = exp2_taylor<12>(y - (shifted - magic));
         const int n = __double2loint(shifted) + kFraction;
         const double w = __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
-        if (top == INFINITY) return x == top ? static_cast<double>(1ull << kFraction) : 0.0;      // (of several: equal)
+        if (x == top) return static_cast<double>(1ull << kFraction);   // (infinite ones, too: y is not a number then)
         return y >= -static_cast<double>(kFraction) ? w : 0.0;         // (else `w` may be anything)
     }
     __device__ __forceinline__ static u64 rounded(double scaled) {
@@ -353,6 +351,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
     pdl_launch_dependents();
     if (tid == 0) {
         mbar_init(smem_u32(&s.loaded), 1);
+        s.bin_count = 0;
         mbar_fence_init();
     }
     pdl_wait();
@@ -481,9 +480,11 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         return z;
     };
     bool cut_known = false;                  // top-p's, in s.cut_key and s.tie_cut
+    int bin_count = 0;                       // tokens of its bin in this CTA, in s.bin_list
     const bool filtered = k > 0 || p < 1.0f || bound > 0.0;
     // ---- top-p over the whole row: its mass, and the bin of its cut
     u64 whole = 0, bin_above = 0, target = 0;
+    u64 above_here = 0;                      // of that, this thread's share of what its CTA has above the bin
     unsigned bin_lo = 0, bin_hi = 0;
     if (k == 0 && p < 1.0f) {
         // exact sums by 32-bit additions: a weight in three pieces of 15 bits (fewer than 2^17 of them a bin and CTA), most of
@@ -502,13 +503,14 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         });
         cluster.sync();
         // a CTA adds its share of the bins up, then all of them learn each share's mass, then where the cut lies
-        constexpr int EACH = kMassBins / kThreads;
+        constexpr int EACH = kMassBins / kThreads;                   // bins of a thread at most
         const int share = kMassBins / static_cast<int>(ranks);       // (128 to 2,048)
+        const int each = max(share / kThreads, 1);
         u64 m[EACH] = {}, sum_m = 0;
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
-            const int bin = EACH * tid + e;
-            if (bin < share)
+            const int bin = each * tid + e;
+            if (e < each && bin < share)
                 for (unsigned c = 0; c < ranks; ++c) {
                     const unsigned* other = cluster.map_shared_rank(&s.pieces[0][0], c) + rank * share + bin;
 #pragma unroll
@@ -535,7 +537,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
             u64 in_front_of = of_the_cut + incl - sum_m;
 #pragma unroll
             for (int e = 0; e < EACH; ++e) {
-                if (m[e] && in_front_of <= target) atomicMax(&s.cross_bin, EACH * tid + e);
+                if (m[e] && in_front_of <= target) atomicMax(&s.cross_bin, each * tid + e);
                 in_front_of += m[e];
             }
             __syncthreads();
@@ -543,7 +545,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
             in_front_of = of_the_cut + incl - sum_m;
 #pragma unroll
             for (int e = 0; e < EACH; ++e) {
-                if (EACH * tid + e == cross) s.cross_above = in_front_of;
+                if (e < each && each * tid + e == cross) s.cross_above = in_front_of;
                 in_front_of += m[e];
             }
             if (warp == 0) {
@@ -562,9 +564,14 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
                 *cluster.map_shared_rank(&s.lo, tid) = found_lo;
                 *cluster.map_shared_rank(&s.hi, tid) = found_hi;
                 *cluster.map_shared_rank(&s.cross_above, tid) = found;
+                *cluster.map_shared_rank(&s.cross_bin, tid) = static_cast<int>(rank) * share + cross;
             }
         }
-        cluster.sync();                      // (nobody reads the pieces any more)
+        cluster.sync();                      // (nobody reads another CTA's pieces any more)
+        for (int bin = tid; bin < s.cross_bin; bin += kThreads)
+#pragma unroll
+            for (int q = 0; q < 3; ++q) above_here += static_cast<u64>(s.pieces[q][bin]) << (15 * q);
+        __syncthreads();
         bin_lo = s.lo;
         bin_hi = s.hi == 0x7fffffffu ? s.hi - 1 : s.hi;      // (the key of -0, which no logit has: as a float it equals 0)
         bin_above = s.cross_above;
@@ -581,37 +588,31 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
             floor_key = max(floor_key, s.key[0]);
             __syncthreads();
         }
-        // counted and listed: the survivors, and where top-p's bin is known its tokens (x, y)
+        // counted and listed: the survivors, in the order of indices, and where top-p's bin is known its tokens
         const unsigned bin_top = k == 0 && p < 1.0f ? bin_hi : 0u;
-        uint2 mine = make_uint2(0, 0);
+        unsigned mine = 0;
         const bool take_all = floor_key <= key_of(-INFINITY);        // (NaN, too)
         const float floor_x = value_of(max(floor_key, key_of(-INFINITY)));
         const float bin_lo_x = bin_top ? value_of(max(bin_lo, key_of(-INFINITY))) : INFINITY, bin_hi_x = bin_top ? value_of(bin_hi) : -INFINITY;
         auto in_all = [&](float x) { return x >= floor_x || take_all; };
         auto in_bin = [&](float x) { return x >= bin_lo_x && x <= bin_hi_x; };      // (not NaN: it has no weight)
-        each_logit(my_seg, mine_n, lane, [&](int, float x) {
-            mine.x += in_all(x) ? 1u : 0u;
-            mine.y += in_bin(x) ? 1u : 0u;
-        });
-        mine.x = __reduce_add_sync(0xffffffffu, mine.x);
-        mine.y = __reduce_add_sync(0xffffffffu, mine.y);
-        if (lane == 0) {
-            s.key[warp] = mine.x;
-            s.at[warp] = mine.y;
-        }
-        __syncthreads();
-        uint2 before = make_uint2(0, 0), here = make_uint2(0, 0);
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) {
-                before.x += s.key[w];
-                before.y += s.at[w];
+        each_logit(my_seg, mine_n, lane, [&](int i, float x) {
+            mine += in_all(x) ? 1u : 0u;
+            if (in_bin(x)) {
+                const unsigned slot = atomicAdd(&s.bin_count, 1u);
+                if (slot < kBinListed) s.bin_list[slot] = Token{key_of(logit_of(x)), lo_i + i};
             }
+        });
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        if (lane == 0) s.key[warp] = mine;
+        __syncthreads();
+        unsigned before = 0;
+        uint2 here = make_uint2(0, s.bin_count);                     // (survivors, tokens of the bin)
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += s.key[w];
             here.x += s.key[w];
-            here.y += s.at[w];
         }
-        const bool list_all = here.x <= kListed, list_bin = here.y <= kBinListed;
-        if ((list_all && mine.x) || (list_bin && mine.y)) {
-            // in the order of indices
+        if (here.x <= kListed && mine) {
             for (int i0 = 0; i0 < mine_n; i0 += 128) {
                 float x[4];
                 bool in = false;
@@ -619,25 +620,16 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
                 for (int e = 0; e < 4; ++e) {
                     const int i = i0 + 32 * e + lane;
                     x[e] = i < mine_n ? to_float(my_seg[i]) : 0.f;
-                    in = in || (i < mine_n && (in_all(x[e]) || in_bin(x[e])));
+                    in = in || (i < mine_n && in_all(x[e]));
                 }
                 if (!__any_sync(0xffffffffu, in)) continue;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = i0 + 32 * e + lane;
-                    const Token token{key_of(logit_of(x[e])), lo_i + i};
-                    if (list_all) {
-                        const bool hit = i < mine_n && in_all(x[e]);
-                        const unsigned hits = __ballot_sync(0xffffffffu, hit);
-                        if (hit) s.list[before.x + __popc(hits & ((1u << lane) - 1))] = token;
-                        before.x += __popc(hits);
-                    }
-                    if (list_bin) {
-                        const bool hit = i < mine_n && in_bin(x[e]);
-                        const unsigned hits = __ballot_sync(0xffffffffu, hit);
-                        if (hit) s.bin_list[before.y + __popc(hits & ((1u << lane) - 1))] = token;
-                        before.y += __popc(hits);
-                    }
+                    const bool hit = i < mine_n && in_all(x[e]);
+                    const unsigned hits = __ballot_sync(0xffffffffu, hit);
+                    if (hit) s.list[before + __popc(hits & ((1u << lane) - 1))] = Token{key_of(logit_of(x[e])), lo_i + i};
+                    before += __popc(hits);
                 }
             }
         }
@@ -648,8 +640,8 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
             n += s.listed[c].x;              // (fewer than 2^20 together)
             n_bin += s.listed[c].y;
         }
-        // all of them in the first CTA, in the order of indices
-        auto gather = [&](bool bins, Token* to, unsigned count) {
+        // the first CTA's share of a list in all CTAs: `take` (place, token)
+        auto gather = [&](bool bins, unsigned count, auto take) {
             for (unsigned i = tid; rank == 0 && i < count; i += kThreads) {
                 unsigned c = 0, from = 0;
                 for (unsigned end = bins ? s.listed[0].y : s.listed[0].x; i >= end; end += bins ? s.listed[c].y : s.listed[c].x) {
@@ -657,16 +649,13 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
                     ++c;
                 }
                 const Token* other = bins ? cluster.map_shared_rank(s.bin_list, c) : cluster.map_shared_rank(s.list, c);
-                to[i] = other[i - from];
+                take(i, other[i - from]);
             }
         };
         if (n > kListed && bin_top && n_bin <= kBinListed) {
             // ---- the first CTA finds top-p's cut among the tokens of its bin
-            gather(true, s.bin_all, n_bin);
+            gather(true, n_bin, [&](unsigned i, Token t) { s.bin_order[i] = (static_cast<u64>(t.key) << 32) | (0xffffffffu - t.at); });
             if (rank == 0) {
-                __syncthreads();
-                for (int i = tid; i < static_cast<int>(n_bin); i += kThreads)
-                    s.bin_order[i] = (static_cast<u64>(s.bin_all[i].key) << 32) | (0xffffffffu - i);
                 __syncthreads();
                 sort_descending(s.bin_order, static_cast<int>(n_bin));
                 u64 w[2], sum;
@@ -677,17 +666,18 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
                 const int kept = __syncthreads_count(w[0] && bin_above + incl - w[0] - w[1] <= target) +
                                  __syncthreads_count(w[1] && bin_above + incl - w[1] <= target);
                 if (tid < static_cast<int>(ranks)) {
-                    const Token last = s.bin_all[0xffffffffu - static_cast<unsigned>(s.bin_order[max(kept, 1) - 1])];
-                    *cluster.map_shared_rank(&s.cut_key, tid) = last.key;
-                    *cluster.map_shared_rank(&s.tie_cut, tid) = last.at;
+                    const u64 last = s.bin_order[max(kept, 1) - 1];
+                    *cluster.map_shared_rank(&s.cut_key, tid) = static_cast<unsigned>(last >> 32);
+                    *cluster.map_shared_rank(&s.tie_cut, tid) = static_cast<int>(0xffffffffu - static_cast<unsigned>(last));
                 }
             }
             cluster.sync();
             cut_known = true;
+            bin_count = static_cast<int>(here.y);
         }
         if (n <= kListed) {
             // ---- the first CTA takes it from here
-            gather(false, all_of, n);
+            gather(false, n, [&](unsigned i, Token t) { all_of[i] = t; });
             cluster.sync();                  // (the others' lists have been read)
             if (rank != 0) return;
             const int count = static_cast<int>(n);
@@ -794,6 +784,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         }
         __syncthreads();
         if (s.lo > cut_key) {
+            cut_known = false;
             cut_key = s.lo;
             ties = ties_kept = 0;
             tie_cut = 0x7fffffff;
@@ -839,6 +830,24 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         return x > cut_x || (x == cut_x && i <= tie_cut) ? heat.weight(x) : 0ull;
     };
 
+    // Where the cut lies in a bin whose tokens are listed, the bins above it say what this CTA keeps: the row's mass is
+    // known, and only a CTA on which a number falls looks for its token.
+    u64 z = 0, from = 0;
+    if (cut_known) {
+        u64 mine = above_here;
+        for (int i = tid; i < bin_count; i += kThreads) {
+            const Token token = s.bin_list[i];
+            mine += kept_weight(token.at, value_of(token.key));
+        }
+        z = cluster_sum(mine, s.total);
+        for (unsigned c = 0; c < rank; ++c) from += s.total[c];
+        bool some = false;
+        for (int j = tid; j < draws; j += kThreads) {
+            const u64 goal = drawn_mass(uniform[draw0 + j], z);
+            some = some || (goal >= from && goal < from + s.total[rank]);
+        }
+        if (!__syncthreads_or(some)) return;
+    }
     // ---- masses: a lane's are those of a contiguous block of its warp's segment (an odd number of tokens: no two lanes
     // of a warp in one bank)
     const int block_n = ((seg + 31) / 32) | 1;
@@ -846,9 +855,14 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
     u64 mine = 0;
     for (int i = b0; i < b1; ++i) mine += kept_weight(lo_i + i, to_float(my_seg[i]));
     __syncthreads();                         // (warp_sum may still be read)
-    const u64 z = cluster_sum(mine, s.total);
-    u64 from = 0;
-    for (unsigned c = 0; c < rank; ++c) from += s.total[c];
+    if (cut_known) {
+        const u64 sum = warp_sum64(mine);
+        if (lane == 0) s.warp_sum[warp] = sum;
+        __syncthreads();
+    } else {
+        z = cluster_sum(mine, s.total);
+        for (unsigned c = 0; c < rank; ++c) from += s.total[c];
+    }
     for (int w = 0; w < warp; ++w) from += s.warp_sum[w];
     from += warp_scan64(mine, lane) - mine;  // what lies in front of this lane's block
     // ---- the draws: each is taken by the warp on whose segment its number falls
