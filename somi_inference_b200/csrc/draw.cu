@@ -896,7 +896,9 @@ int launch_draw(const void* logits, long long stride, int rows, int V, const Set
                 int* out, float* prob, cudaStream_t stream) {
     int ranks = 1;
     const auto bytes_of = [&](int n) { return static_cast<long long>(V) / n * static_cast<long long>(sizeof(T)); };
-    while (ranks < 8 && V > ranks * 4096 && !(rows * ranks >= 256 && bytes_of(ranks) <= 78 * 1024)) ranks *= 2;
+    // (16 CTAs a row while the rows' clusters find room beside each other: 152,064 logits with top-k, top-p and min-p, 1 row 11.7 us,
+    // with 8 13.1; 12 rows 14.4 and 15.8; 16 rows 20.5 and 16.5)
+    while (ranks < (rows <= 12 ? kMaxCluster : 8) && V > ranks * 4096 && !(rows * ranks >= 256 && bytes_of(ranks) <= 78 * 1024)) ranks *= 2;
     const int most = 192 * 1024;             // bytes of a slice beside the static shared memory
     const auto segment = [&](int n) { return ((V + n * kWarps - 1) / (n * kWarps) + 7) / 8 * 8; };
     while (ranks < kMaxCluster && static_cast<long long>(segment(ranks)) * kWarps * sizeof(T) > most) ranks *= 2;
