@@ -382,7 +382,7 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         const uint32_t s_addr = tmem_s + x * kTile + lane_addr;
         const uint32_t o_addr = tmem_o + lane_addr;
         bool ok = true;
-        // this warp's share of a piece's query rows into shared memory
+        // this warp's share of a piece's query rows into shared memory: on their way, and there
         auto load_queries = [&](const PieceNote& p) {
             const int rows_w = p.wide ? 32 : 16, r0 = p.wide ? quarter * 32 : warp * 16;
             unsigned char* to = p.wide && x ? Q1 : Qs;
@@ -398,8 +398,10 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                                 q + (token0 + t) * q_stride + static_cast<size_t>(p.kvh * b.per + r - t * b.per) * HD + chunk * 8, 16);
                 }
                 cp_async_commit();
-                cp_async_wait<0>();
             }
+        };
+        auto announce_queries = [&]() {
+            cp_async_wait<0>();
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&q_full));
@@ -412,7 +414,10 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             ok = tail.softmax_failed[n & 1] == 0;
         };
         ok = get_piece(0, ok);
-        if (ok && ring[0].tiles >= 0) load_queries(ring[0]);
+        if (ok && ring[0].tiles >= 0) {
+            load_queries(ring[0]);
+            announce_queries();
+        }
         together(1);
         for (int n = 0; ok; ++n) {
             const PieceNote& p = ring[n % kPieces];
@@ -538,9 +543,11 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             ok = mbar_wait(smem_u32(&o_done), n & 1, ok ? 400000 : 1) && ok;
             __syncwarp();
             t5::fence_after();
-            // the next piece's queries, so that its first scores are computed while this one's rows are written
+            // the next piece's queries are on their way while the first half of this one's outputs is written, and its first
+            // scores are computed during the second
             ok = get_piece(n + 1, ok);
-            if (ok && ring[(n + 1) % kPieces].tiles >= 0) load_queries(ring[(n + 1) % kPieces]);
+            bool queries = ok && ring[(n + 1) % kPieces].tiles >= 0;
+            if (queries) load_queries(ring[(n + 1) % kPieces]);
 
             const int head = p.kvh * b.per + row % b.per, token = p.token0 + my_token;
             const bool mine = row < live;
@@ -553,6 +560,10 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                     for (int c = 0; c < HD / 32; ++c) {
                         // (the loads are the whole warp's: whatever a compiler makes of the condition below, it meets here)
                         __syncwarp();
+                        if (c == HD / 64 && queries) {
+                            announce_queries();
+                            queries = false;
+                        }
                         float v[32];
                         t5::ld32(o_addr + x * kTile + c * 32, v);
                         if (mine) {
@@ -577,6 +588,10 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                     for (int c = 0; c < HD / 32; ++c) {
                         const uint32_t col = x * (HD / 2) + c * 16;
                         __syncwarp();
+                        if (c == HD / 64 && queries) {
+                            announce_queries();
+                            queries = false;
+                        }
                         float y[16];
                         ld16(o_addr + col, y);
 #pragma unroll
@@ -594,6 +609,7 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
                     }
                 }
             }
+            if (queries) announce_queries();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&piece_empty[n % kPieces]));
             t5::fence_before();
