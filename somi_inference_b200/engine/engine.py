@@ -284,6 +284,8 @@ class Engine:
         attend to them once for all.  Returns how many positions `request` has now (0: less than a page is
         shared, and nothing was registered); its next tokens continue from there.  Models with windows or
         states refuse."""
+        if not self.cache.is_registered(of):
+            raise ValueError(f"request {of!r} holds nothing that could be shared")
         cached = self.cache.length(of)
         if tokens is not None and not 0 <= tokens <= cached:
             raise ValueError(f"{tokens} positions of {of!r} are wanted, {cached} are cached")

@@ -155,8 +155,9 @@ def test_forked_requests_continue_like_whole_ones(root):
     prompt = random_tokens(37, cfg["vocab_size"], 1)
     eng.step([StepEntry("p", prompt, [36])])
     assert eng.fork("none", "p", 15) == 0 and not eng.has("none")
-    with pytest.raises(ValueError):
-        eng.fork("none", "p", 38)
+    for of, n in (("p", 38), ("p", -1), ("unknown", 16)):
+        with pytest.raises(ValueError):
+            eng.fork("none", of, n)
     ends = {f"r{i}": random_tokens(n, cfg["vocab_size"], 2 + i) for i, n in enumerate((7, 1, 20))}
     assert [eng.fork(r, "p") for r in ends] == [32] * 3
     assert eng.length("r1") == 32 and eng.cache.free_pages() == [12 - 3]

@@ -215,3 +215,52 @@ def test_no_rows_or_draws_is_no_launch(ops):
     one = torch.ones(1, device="cuda")
     ops.draw_tokens(torch.empty(1, 9, device="cuda"), f.view(1, 0), one, one.int(), one, one, i.view(1, 0))
     assert ops.launches == before
+
+
+@pytest.mark.parametrize("rows", [1, 13, 260])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_flat_rows_of_any_number_with_many_draws(ops, rows, dtype):
+    """top-p alone among nearly equal weights: numbers fall on every part of a row, however many CTAs share it."""
+    g = torch.Generator().manual_seed(rows)
+    x = (torch.randn(rows, 70001, generator=g) * 0.7).to(dtype)
+    u = torch.rand(rows, 33, generator=g)
+    u[:, 0], u[:, 1] = 0.0, 1.0 - 2.0 ** -24
+    settings = [(0.9, -1, (0.9, 0.3, 0.99)[r % 3], 0.0) for r in range(rows)]
+    if rows < 260:
+        check(ops, x, settings, u)
+        return
+    some = [0, 1, 2, 77, 128, 259]
+    args = [torch.tensor(c).cuda() for c in zip(*settings)]
+    out, prob = torch.empty(u.shape, dtype=torch.int32, device="cuda"), torch.empty(u.shape, device="cuda")
+    ops.draw_tokens(x.cuda(), u.cuda(), args[0].float(), args[1].int(), args[2].float(), args[3].float(), out, prob=prob)
+    alone = check(ops, x[some], [settings[r] for r in some], u[some])
+    assert torch.equal(out[some], alone)
+    ops.check_errors()
+
+
+def test_two_calls_at_once(ops):
+    g = torch.Generator().manual_seed(3)
+    calls = []
+    for i, (rows, V) in enumerate(((4, 152064), (60, 32000))):
+        n = len(SETTINGS)
+        cols = [torch.tensor([SETTINGS[(r + i) % n][c] for r in range(rows)]).cuda() for c in range(4)]
+        calls.append((torch.randn(rows, V, generator=g).mul(3).cuda(), torch.rand(rows, 3, generator=g).cuda(), cols[0].float(),
+                      cols[1].int(), cols[2].float(), cols[3].float()))
+
+    def run(c):
+        out, prob = torch.empty(c[1].shape, dtype=torch.int32, device="cuda"), torch.empty(c[1].shape, device="cuda")
+        ops.draw_tokens(*c, out, prob=prob)
+        return out, prob
+
+    alone = [run(c) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for c, s in zip(calls, streams):
+            with torch.cuda.stream(s):
+                got.append(run(c))
+    torch.cuda.synchronize()
+    for i, (out, prob) in enumerate(got):
+        assert torch.equal(out, alone[i % 2][0]) and torch.equal(prob, alone[i % 2][1])
+    ops.check_errors()

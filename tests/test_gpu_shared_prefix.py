@@ -185,3 +185,39 @@ def test_no_rows_is_no_launch(ops):
     ops.shared_prefix_attention(empty, case.keys, case.values, case.table[:0], ints[:0], ints[:0], ints, 4, 2, 64, 1.0,
                                 torch.empty((0, 256), device="cuda"))
     assert ops.launches == before
+
+
+@pytest.mark.parametrize("dtype,heads,members", [(torch.bfloat16, (28, 4, 128), [0, 3, 70, 200]), (torch.bfloat16, (14, 2, 64), [5, 20]),
+                                                 (torch.float32, (14, 2, 64), [0, 3, 70])])
+def test_a_cache_whose_offsets_pass_32_bits(ops, dtype, heads, members):
+    """The pages that are read lie behind 2^31 elements; nothing else of the cache is (it holds whatever was there)."""
+    nq, nkv, hd = heads
+    case = Case(nq, nkv, hd, 64, [(300, ones(*members))], dtype, seed=21)
+    in_front = (1 << 31) // (nkv * 64 * hd) + 3
+    for name in ("keys", "values"):
+        small = getattr(case, name)
+        big = torch.empty((in_front + small.shape[0],) + small.shape[1:], dtype=dtype, device="cuda")
+        big[in_front:] = small
+        setattr(case, name, big)
+    case.table = torch.where(case.table >= 0, case.table + in_front, case.table)
+    case.check(case.call(ops), sums(case))
+
+
+def test_two_calls_at_once(ops):
+    """On two streams, each with its own workspace: the same bits as one behind the other."""
+    cases = [Case(28, 4, 128, 16, [(2000 + 16 * i, ones(*range(0, 130, 5)))], torch.bfloat16, seed=22 + i) for i in range(2)]
+    cases += [Case(14, 2, 64, 16, [(900, ones(3, 9))], torch.bfloat16, seed=24)]
+    alone = [c.call(ops).clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = [[torch.full_like(c.out, 3.0) for _ in range(6)] for c in cases]
+    torch.cuda.synchronize()
+    for i in range(6):
+        for c, s, o in zip(cases, streams, outs):
+            with torch.cuda.stream(s):
+                c.call(ops, out=o[i])
+    torch.cuda.synchronize()
+    for want, o in zip(alone, outs):
+        for got in o:
+            assert torch.equal(got, want)
+    ops.check_errors()
