@@ -26,7 +26,12 @@
 // span the 30.5 temperatures in which weights do not vanish), then the keys (the order-preserving integer image of a
 // float) that lie in the bin of the cut, until a bin is one key (top-p's bin, where it holds no more than `kListed`,
 // is sorted in one CTA instead); what is kept is then a key and an index up to which logits equal to it are kept, and
-// weights are computed a second time to find where the numbers fall.
+// weights are computed a second time to find where the numbers fall (where top-p's bin was sorted, the bins above it tell every CTA
+// what it keeps, and only one on which a number falls weighs again).
+//
+// Measured (152,064 logits): 1 row with all filters 10.8 us (a chain of exchanges and a sort; HBM would need 0.1), 8 rows without
+// any 13.2, 64 rows of mixed settings 57.6, 256 bfloat16 rows with top-p 281: about 90 instructions a weight and
+// token at 2.7 of 4 issue slots a cycle; the float64 pipe is a quarter busy.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -43,6 +48,8 @@ constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kMaxCluster 
 constexpr int kMassBins = 2048;              // of the masses that top-p cuts
 constexpr int kListed = 2048;                // survivors that one CTA takes
 constexpr int kBinListed = 1024;             // tokens of top-p's bin that one CTA takes
+constexpr int kCounted = 2 * 16 * 128;       // values of 16-bit logits that are counted: signs, exponents (2^-8 to 2^8), mantissas
+constexpr unsigned kCountedFrom = 119u << 7;
 constexpr int kFraction = 44;                // a weight is an integer multiple of 2^-44
 typedef unsigned long long u64;
 
@@ -492,15 +499,43 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         for (int i = tid; i < 3 * kMassBins; i += kThreads) (&s.pieces[0][0])[i] = 0;
         if (tid == 0) s.cross_bin = -1;
         __syncthreads();
-        each_logit(my_seg, mine_n, lane, [&](int, float x) {
+        auto add_to_bin = [&](float x, unsigned times) {
             const u64 w = heat.weight(x);    // (NaN: none)
             if (!w) return;
             const int bin = heat.bin<kMassBins>(x);
             const unsigned a = static_cast<unsigned>(w) & 32767u, b = static_cast<unsigned>(w >> 15) & 32767u, c = static_cast<unsigned>(w >> 30);
-            if (a) atomicAdd(&s.pieces[0][bin], a);
-            if (b) atomicAdd(&s.pieces[1][bin], b);
-            if (c) atomicAdd(&s.pieces[2][bin], c);
-        });
+            if (a) atomicAdd(&s.pieces[0][bin], a * times);
+            if (b) atomicAdd(&s.pieces[1][bin], b * times);
+            if (c) atomicAdd(&s.pieces[2][bin], c * times);
+        };
+        bool counted = false;
+        if constexpr (sizeof(T) == 2) {
+            // Logits of 16 bits have few values: those of sixteen exponents are counted (two counters of 16 bits a word), and a
+            // weight is computed once a value; others, next to zero or far from it, are weighed one by one.
+            __shared__ unsigned counts[kCounted / 2];
+            counted = slice_n >= 4 * kCounted && slice_n < 65536;
+            if (counted) {
+                for (int i = tid; i < kCounted / 2; i += kThreads) counts[i] = 0;
+                __syncthreads();
+                each_logit(my_seg, mine_n, lane, [&](int, float x) {
+                    const unsigned bits = __float_as_uint(x), at = ((bits >> 16) & 0x7fffu) - kCountedFrom;
+                    if (at < kCounted / 2) {
+                        // (a value and its negative share a word)
+                        atomicAdd(&counts[at], (bits >> 31) ? 65536u : 1u);
+                    } else {
+                        add_to_bin(x, 1u);
+                    }
+                });
+                __syncthreads();
+                for (int i = tid; i < kCounted / 2; i += kThreads) {
+                    const unsigned n = counts[i];
+                    const float x = __uint_as_float((i + kCountedFrom) << 16);
+                    if (n & 0xffffu) add_to_bin(x, n & 0xffffu);
+                    if (n >> 16) add_to_bin(-x, n >> 16);
+                }
+            }
+        }
+        if (!counted) each_logit(my_seg, mine_n, lane, [&](int, float x) { add_to_bin(x, 1u); });
         cluster.sync();
         // a CTA adds its share of the bins up, then all of them learn each share's mass, then where the cut lies
         constexpr int EACH = kMassBins / kThreads;                   // bins of a thread at most
