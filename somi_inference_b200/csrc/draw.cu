@@ -30,8 +30,8 @@
 // what it keeps, and only one on which a number falls weighs again).
 //
 // Measured (152,064 logits): 1 row with all filters 10.8 us (a chain of exchanges and a sort; HBM would need 0.1), 8 rows without
-// any 13.2, 64 rows of mixed settings 57.6, 256 bfloat16 rows with top-p 281: about 90 instructions a weight and
-// token at 2.7 of 4 issue slots a cycle; the float64 pipe is a quarter busy.
+// any 13.2, 64 rows of mixed settings 57.6 (about 90 instructions a weight and token), 256 bfloat16 rows with top-p 217 (weighed once a
+// value, 281 once a token): instructions at 2.1 of 4 issue slots a cycle, and barriers.
 #include <cooperative_groups.h>
 
 #include <algorithm>
