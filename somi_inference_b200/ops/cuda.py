@@ -756,6 +756,9 @@ class CudaOps:
     # (2^23) 15.0 and 17.2, 8 behind 8,192 (2^24) 25.8 and 17.8, 64 behind 2,048 (2^25) 44.8 and 25.3; what every request
     # has read once lies in L2, and a step takes the longer way of parts, products of whole tiles and a merge.
     SHARED_PREFIX_VALUES = 1 << 25
+    # ... and positions a request of the step, since each has a piece of its own, whose chain is longer than a split of the usual
+    # kernel: beside 16 behind 4,096, 24 requests of 4,000 that share nothing 63.5 us and 52.2, 64 of 500 36.1 and 45.5
+    SHARED_PREFIX_POSITIONS = 1024
     # Short portions fill tiles of their own badly: 4 portions of 16 behind 512 (2^19) 16.6 us and 16.6, 2 behind 2,048
     # (2^20) 40.9 and 19.1, 64 of 2 behind 64 (2^20) 72.5 and 19.2.  Longer ones gain only behind much longer prefixes:
     # of 64, 16 behind 176 33.8 and 48.6, 8 behind 1,024 40.3 and 38.4, 16 behind 4,096 229.7 and 99.2; of 128, 16 behind
@@ -769,7 +772,7 @@ class CudaOps:
             return False
         portions, values = batch.num_prefill_requests, nkv * hd << saved_bits
         if portions == 0:
-            pays = values >= self.SHARED_PREFIX_VALUES
+            pays = values >= self.SHARED_PREFIX_VALUES and 1 << saved_bits >= self.SHARED_PREFIX_POSITIONS * batch.num_requests
         else:
             mean = batch.num_prefill_tokens / portions
             pays = values >= self.SHARED_PREFIX_VALUES_PORTIONS and (

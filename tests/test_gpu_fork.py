@@ -32,6 +32,7 @@ def engine(d, dtype="bfloat16", saves=1):
     from somi_inference_b200 import Engine
     from somi_inference_b200.ops import CudaOps
     ops = CudaOps()
+    ops.SHARED_PREFIX_POSITIONS = 0
     ops.SHARED_PREFIX_VALUES = ops.SHARED_PREFIX_VALUES_PORTIONS = saves          # (the tests' prefixes are short)
     calls = []
     inner = ops.shared_prefix_attention

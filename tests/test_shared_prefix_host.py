@@ -93,3 +93,25 @@ def test_what_the_launcher_refuses_is_an_error(ops):
     ops._shared_attention = lambda *a: cuda.ERR_UNSUPPORTED
     with pytest.raises(KernelError, match="not supported"):
         ops.shared_prefix_attention(**arguments())
+
+
+def test_the_rule_of_a_step(ops):
+    """Which steps of forked requests go the shared way: by type, head sizes and what it saves."""
+    from types import SimpleNamespace
+    ops.use_shared_prefix = True
+    ops.lib.somi_shared_attention_tc_takes = lambda nq, nkv, hd, page: int(hd in (64, 128) and 128 % page == 0)
+    rows = {d: torch.zeros(2, 36 * 128, dtype=d) for d in (torch.bfloat16, torch.float32)}
+
+    def pays(saved, singles=0, portions=0, tokens=0, dtype=torch.bfloat16, page=16, hd=128, qkv=None):
+        batch = SimpleNamespace(num_requests=singles + portions, num_prefill_requests=portions, num_prefill_tokens=tokens,
+                                num_tokens=singles + tokens)
+        return ops.shared_prefix_pays(saved.bit_length(), batch, 28, 4, hd, rows[dtype] if qkv is None else qkv, page)
+
+    assert pays(63 * 2048, 64) and pays(7 * 8192, 8) and not pays(7 * 2048, 8) and not pays(63 * 512, 64)
+    assert not pays(15 * 4096, 80) and pays(15 * 4096, 40)         # beside many that share nothing
+    assert not pays(63 * 2048, 64, dtype=torch.float32) and not pays(63 * 2048, 64, page=24) and not pays(63 * 2048, 64, hd=96)
+    assert not pays(63 * 2048, 64, qkv=rows[torch.bfloat16][:, :-4]) and not pays(10 ** 9, 5000)
+    assert pays(3 * 2048, 0, 4, 64) and not pays(15 * 64, 0, 16, 64) and pays(15 * 4096, 0, 16, 16 * 64)
+    assert not pays(15 * 176, 0, 16, 16 * 64) and not pays(15 * 4096, 0, 16, 16 * 200)
+    ops.use_shared_prefix = False
+    assert not pays(63 * 2048, 64)
