@@ -36,9 +36,10 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
     pdl_launch_dependents();
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     __shared__ GroupScratch group_scratch;
-    const Groups groups = hold_groups(b, group_scratch);      // [descriptor]
+    Raw raw;
+    const Groups groups = hold_groups<kThreads>(b, group_scratch, raw);      // [descriptor]
     __shared__ unsigned owned[kOwned];
-    const Range range = find_range<kThreads>(b, groups, scratch, owned);
+    const Range range = find_range<kThreads>(b, groups, raw, scratch, owned);
     pdl_wait();
 
     Walk walk(range);

@@ -37,8 +37,9 @@ shared_rows_kernel(const Batch b, const __nv_bfloat16* __restrict__ q, long long
     unsigned char* ring = smem + warp * STAGES * 2 * TILE;
 
     pdl_launch_dependents();
-    const Groups groups = hold_groups(b, group_scratch);              // [descriptor]
-    const Range range = find_range<kFewThreads>(b, groups, scratch, owned);
+    Raw raw;
+    const Groups groups = hold_groups<kFewThreads>(b, group_scratch, raw);              // [descriptor]
+    const Range range = find_range<kFewThreads>(b, groups, raw, scratch, owned);
     pdl_wait();
 
     Walk walk(range);

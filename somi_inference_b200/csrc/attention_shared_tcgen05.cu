@@ -149,38 +149,35 @@ shared_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
 
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) {
-        for (int w = 0; w < 2; ++w) {
-            for (int s = 0; s < kMaxK; ++s) {
-                mbar_init(smem_u32(&k_full[w][s]), 1);
-                mbar_init(smem_u32(&k_empty[w][s]), 1);
-            }
-            for (int s = 0; s < kMaxV; ++s) {
-                mbar_init(smem_u32(&v_full[w][s]), 1);
-                mbar_init(smem_u32(&v_empty[w][s]), 1);
-            }
-            mbar_init(smem_u32(&s_full[w]), 1);
-            mbar_init(smem_u32(&p_full[w]), 4);                       // one arrival per warp of the group
-        }
+    // (a thread each: one alone would keep the others waiting)
+    if (tid < 4 * (kMaxK + kMaxV)) {
+        unsigned long long* const barriers = &k_full[0][0];           // k_full, k_empty, v_full, v_empty, one behind the other
+        mbar_init(smem_u32(barriers + tid), 1);
+    } else if (tid >= 64 && tid < 64 + kPieces) {
+        mbar_init(smem_u32(&piece_full[tid - 64]), 1);
+        mbar_init(smem_u32(&piece_empty[tid - 64]), 11);              // 8 softmax warps, 2 producers, the issuer
+    } else if (tid == 96 || tid == 97) {
+        mbar_init(smem_u32(&s_full[tid - 96]), 1);
+        mbar_init(smem_u32(&p_full[tid - 96]), 4);                    // one arrival per warp of the group
+    } else if (tid == 128) {
         mbar_init(smem_u32(&q_full), 8);
         mbar_init(smem_u32(&o_done), 1);
         mbar_init(smem_u32(&mode_done), 1);
-        for (int s = 0; s < kPieces; ++s) {
-            mbar_init(smem_u32(&piece_full[s]), 1);
-            mbar_init(smem_u32(&piece_empty[s]), 11);                 // 8 softmax warps, 2 producers, the issuer
-        }
-        mbar_fence_init();
         failed_s = smem_u32(base) & 1023 ? 1 : 0;                     // (the swizzled layout needs the alignment)
         tail.softmax_failed[0] = tail.softmax_failed[1] = 0;
     }
+    if (tid < 160) mbar_fence_init();
+    static_assert(4 * (kMaxK + kMaxV) <= 64 && offsetof(Tail, s_full) == 4 * (kMaxK + kMaxV) * sizeof(unsigned long long),
+                  "the rings' barriers lie one behind the other");
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_base_s)),
                      "r"(TmemCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    const Groups groups = hold_groups(b, tail.groups);                // [descriptor]
-    const Range range = find_range<kTcThreads>(b, groups, scratch, tail.owned);   // [descriptor]
+    Raw raw;
+    const Groups groups = hold_groups<kTcThreads>(b, tail.groups, raw);                // [descriptor]
+    const Range range = find_range<kTcThreads>(b, groups, raw, scratch, tail.owned);   // [descriptor]
     t5::fence_before();
     __syncthreads();
     t5::fence_after();

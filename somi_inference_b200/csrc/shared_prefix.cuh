@@ -59,7 +59,7 @@ struct Entry {
     int tiles, unit, units;         // tiles of tokens, keys of a unit, units of an item
     int over;                       // what an item costs beside its units
     __device__ __forceinline__ int cost() const { return units + over; }
-    __device__ __forceinline__ int base(const Batch& b) const { return key_lo / b.align * b.align; }
+    __device__ __forceinline__ int base(const Batch& b) const { return key_lo & -b.align; }
 };
 
 __device__ __forceinline__ int clamped(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -79,8 +79,14 @@ __device__ __forceinline__ int group_of(const Batch& b, const Groups& g, int r) 
     return lo > 0 && r < g.off[lo] ? lo - 1 : -1;
 }
 
-// Everything that lengths lead to stays inside the batch's rows and the table's columns, whatever they hold.
-__device__ __forceinline__ Entry entry_of(const Batch& b, const Groups& gs, int e) {
+// What the arrays say about a request.
+struct Raw { int ctx, first, end; };
+__device__ __forceinline__ Raw raw_of(const Batch& b, int r) {
+    return Raw{ld_step(b.ctx_len + r), token_of(b, r), b.cu_q ? token_of(b, r + 1) : r + 1};
+}
+
+// Everything that lengths lead to stays inside the batch's rows and the table's columns, whatever they hold.  `raw`: of a request's entry.
+__device__ __forceinline__ Entry entry_of(const Batch& b, const Groups& gs, int e, const Raw& raw) {
     Entry x;
     const int span = b.bt_stride * b.page_size;
     if (e < b.G) {
@@ -89,14 +95,14 @@ __device__ __forceinline__ Entry entry_of(const Batch& b, const Groups& gs, int 
         x.first = token_of(b, r0);
         x.tokens = r1 > r0 ? max(token_of(b, r1) - x.first, 0) : 0;
         x.key_lo = 0;
-        x.key_hi = clamped(gs.prefix[e], 0, min(span, max(0, ld_step(b.ctx_len + x.table))));
+        x.key_hi = clamped(gs.prefix[e], 0, span);
         x.pos0 = 0x3fffffff;        // every token sees the whole prefix
     } else {
         const int r = e - b.G, g = group_of(b, gs, r);
         x.table = r;
-        x.first = token_of(b, r);
-        x.tokens = b.cu_q ? max(token_of(b, r + 1) - x.first, 0) : 1;
-        const int ctx = clamped(ld_step(b.ctx_len + r), 0, span);
+        x.first = raw.first;
+        x.tokens = max(raw.end - x.first, 0);
+        const int ctx = clamped(raw.ctx, 0, span);
         x.key_lo = g >= 0 ? clamped(gs.prefix[g], 0, ctx) : 0;
         x.key_hi = min(ctx + x.tokens, span);
         x.pos0 = ctx;
@@ -106,8 +112,11 @@ __device__ __forceinline__ Entry entry_of(const Batch& b, const Groups& gs, int 
     x.over = wide ? b.over_wide : 1;
     const bool some = x.tokens > 0 && x.key_hi > x.key_lo;
     x.tiles = some ? (x.tokens + b.item_tokens - 1) / b.item_tokens : 0;
-    x.units = some ? (x.key_hi - x.base(b) + x.unit - 1) / x.unit : 0;
+    x.units = some ? (x.key_hi - x.base(b) + x.unit - 1) >> (31 - __clz(x.unit)) : 0;
     return x;
+}
+__device__ __forceinline__ Entry entry_of(const Batch& b, const Groups& gs, int e) {
+    return entry_of(b, gs, e, e >= b.G ? raw_of(b, e - b.G) : Raw{0, 0, 0});
 }
 
 // How `total` costs are shared out over `n` CTAs.
@@ -142,10 +151,12 @@ struct GroupScratch {
     int off[kGroupsHeld + 1], prefix[kGroupsHeld + 1];
 };
 
-// All threads of the block, first of all.
-__device__ __forceinline__ Groups hold_groups(const Batch& b, GroupScratch& s) {
+// All threads of the block, first of all.  `raw`: what find_range asks for next, so that it is on its way meanwhile.
+template <int THREADS>
+__device__ __forceinline__ Groups hold_groups(const Batch& b, GroupScratch& s, Raw& raw) {
+    const int i = threadIdx.x, r = i * ((b.G + b.R + THREADS - 1) / THREADS) - b.G;
+    raw = r >= 0 && r < b.R ? raw_of(b, r) : Raw{0, 0, 0};
     if (b.G > kGroupsHeld) return Groups{b.group_off, b.prefix_len};
-    const int i = threadIdx.x;
     if (i <= b.G) s.off[i] = ld_step(b.group_off + i);
     if (i >= 32 && i - 32 < b.G) s.prefix[i - 32] = ld_step(b.prefix_len + i - 32);
     __syncthreads();
@@ -154,14 +165,14 @@ __device__ __forceinline__ Groups hold_groups(const Batch& b, GroupScratch& s) {
 
 // All threads of the block.  owned[k]: where entry blockIdx.x + k gridDim.x begins, whose tokens this CTA notes.
 template <int THREADS>
-__device__ __forceinline__ Range find_range(const Batch& b, const Groups& gs, RangeScratch& s, unsigned* owned) {
+__device__ __forceinline__ Range find_range(const Batch& b, const Groups& gs, const Raw& raw, RangeScratch& s, unsigned* owned) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int E = b.G + b.R, each = (E + THREADS - 1) / THREADS;
     const int e0 = tid * each, e1 = min(e0 + each, E);
     unsigned mine = 0;
     Entry first_entry;
     for (int e = e0; e < e1; ++e) {
-        const Entry x = entry_of(b, gs, e);
+        const Entry x = e == e0 ? entry_of(b, gs, e, raw) : entry_of(b, gs, e);
         if (e == e0) first_entry = x;
         mine += static_cast<unsigned>(x.tiles) * x.cost() * b.nkv;
     }
