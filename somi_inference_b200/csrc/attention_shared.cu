@@ -7,7 +7,7 @@
 // path of float32 and of head sizes and pages that the tensor-core kernel does not take.
 //
 // Measured (float32): 8 requests behind 1,504 positions (14 heads of 64) 19.1 us, a chain of phases (load, scores, softmax, outputs) of
-// one or two tiles a CTA and the merge; portions of 40 of 24 requests behind 4,096 (28 of 128) 1,220 us, 49 TFLOP/s of the 74 that
+// one or two tiles a CTA and the merge; portions of 40 of 24 requests behind 4,096 (28 of 128) 1,192 us, 50 TFLOP/s of the 74 that
 // the FMA pipe reaches.
 #include "mma.cuh"
 #include "shared_prefix.cuh"

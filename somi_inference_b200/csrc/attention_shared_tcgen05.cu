@@ -26,8 +26,8 @@
 // of the first and last tile before they announce the probabilities.  Every wait on an mbarrier is
 // bounded and failure is recorded in an error word.
 //
-// Measured (28 heads of 128 over 4, in a row): 64 requests behind 8,192 positions with 200 of their own 35.5 us, 8 behind 2,048
-// 13.6, portions of 1 to 47 tokens of 24 requests behind 20,000 164 us (920 TFLOP/s).  Long pieces are bound by the softmax
+// Measured (28 heads of 128 over 4, in a row): 64 requests behind 8,192 positions with 200 of their own 35.2 us, 8 behind 2,048
+// 13.3, portions of 1 to 47 tokens of 24 requests behind 20,000 163 us (925 TFLOP/s).  Long pieces are bound by the softmax
 // chain of a tile (load, maximum, 2^x, store: 2.1 us a pair of tiles), short ones by the chain from the block table to the
 // written part (4.5 us, of which the products are a tenth).
 #include "shared_prefix.cuh"

@@ -35,7 +35,7 @@ struct Batch {
     int bt_stride, R, G, T, nq, nkv, per, page_size, num_pages;
     int item_tokens;                // tokens of a tile, at most
     int wide_tokens;                // entries of more tokens than this have units of `unit_wide` keys
-    int unit_narrow, unit_wide, align;
+    int unit_narrow, unit_wide, align;       // keys; powers of two
     int over_wide;                  // what their items cost beside their units (others: 1)
     int block_rows;                 // rows of a CTA's continuation
 };

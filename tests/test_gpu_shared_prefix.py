@@ -221,3 +221,16 @@ def test_two_calls_at_once(ops):
         for got in o:
             assert torch.equal(got, want)
     ops.check_errors()
+
+
+@pytest.mark.parametrize("nq,nkv,hd,page", [(28, 4, 128, 16), (14, 2, 64, 8), (8, 8, 128, 128), (40, 8, 128, 32), (4, 4, 64, 64)])
+def test_many_requests_with_few_keys_of_their_own(ops, nq, nkv, hd, page):
+    """Single tokens with 1 to 64 keys of their own, and more, beside short portions; with a prefix and without one."""
+    own = [0, 1, 5, 31, 32, 33, 62, 63, 64, 65, 130]
+    groups = [(300, ones(*own)), (1000, ones(*own) + [(10, 3), (0, 1), (63, 2)])] + [(129, ones(*own[g % 3:])) for g in range(6)]
+    case = Case(nq, nkv, hd, page, groups, torch.bfloat16, seed=31, loose=ones(*own, 400))
+    case.check(case.call(ops), "bfloat16")
+    case = Case(nq, nkv, hd, page, [(600, ones(*own * 9))], torch.bfloat16, seed=32, loose=ones(*own * 4))
+    case.check(case.call(ops), "bfloat16")
+    again = case.call(ops, out=torch.full_like(case.out, 2.0))
+    assert torch.equal(again, case.out)
