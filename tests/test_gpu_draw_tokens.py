@@ -264,3 +264,28 @@ def test_two_calls_at_once(ops):
     for i, (out, prob) in enumerate(got):
         assert torch.equal(out, alone[i % 2][0]) and torch.equal(prob, alone[i % 2][1])
     ops.check_errors()
+
+
+def test_counted_values_of_16_bits(ops):
+    """Rows long enough for a CTA to count values, and what it does not count: NaN, zeros, values next to zero and far from it."""
+    g = torch.Generator().manual_seed(40)
+    V = 152064
+    x = torch.randn(17, V, generator=g)
+    x[1, ::2] = float("nan")
+    x[2, ::3], x[2, 1::3] = 0.0, -0.0
+    x[3] *= 2.0 ** -9                        # most of them below the least value that is counted
+    x[4] *= 150                              # some above the largest
+    x[5, ::2] = -float("inf")
+    x[6] = (x[6] * 2).round() / 2            # few values, thousands of tokens each
+    x[7] = 1.0
+    x[8] = -300.0 + x[8]
+    x[9, 100:200] = float("inf")
+    x[10] = 2.0 ** -8 * (1 - 2 * torch.randint(0, 2, (V,), generator=g)) * (1 + torch.randint(0, 2, (V,), generator=g) / 128)
+    x[11] = 256.0 - x[11].abs()
+    x[12] = -x[12].abs()
+    x[13] *= 5
+    x = x.bfloat16()
+    u = torch.rand(17, 12, generator=g)
+    for p in (0.3, 0.97):
+        check(ops, x, [((1.0, 0.6, 3.0)[r % 3], -1, p, 0.0 if r % 5 else 1e-4) for r in range(17)], u)
+    ops.check_errors()
