@@ -35,6 +35,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "mma.cuh"
 #include "tma.cuh"
@@ -361,6 +362,9 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
         s.bin_count = 0;
         mbar_fence_init();
     }
+    // (another CTA's shared memory may be written only once that CTA runs: all have said so in front of the first exchange, and
+    // the answer arrives behind the copy)
+    auto running = cluster.barrier_arrive();
     pdl_wait();
     const T* x_row = logits + row * stride + first;
     const int slice_n = max(min(first + kWarps * seg, V) - first, 0);
@@ -426,6 +430,7 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
             }
         }
     }
+    cluster.barrier_wait(std::move(running));                  // every CTA of the cluster has begun
     if (tid < static_cast<int>(ranks)) {
         unsigned best = 0;
         for (int w = 0; w < kWarps; ++w) best = max(best, s.key[w]);
