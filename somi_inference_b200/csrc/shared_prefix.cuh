@@ -40,9 +40,13 @@ struct Batch {
     int block_rows;                 // rows of a CTA's continuation
 };
 
-// The groups' borders and prefixes as a block reads them: its own copies where they are few.
+// The groups' borders and prefixes as a block reads them: its own copies where they are few; else the step's arrays, which are
+// read before the kernels in front have ended, and so through L2.
 struct Groups {
     const int *off, *prefix;
+    bool held;
+    __device__ __forceinline__ int border(int g) const { return held ? off[g] : ld_step(off + g); }
+    __device__ __forceinline__ int shared(int g) const { return held ? prefix[g] : ld_step(prefix + g); }
 };
 
 // What joins the parts: per token, for the prefix and for its own keys, where the item of its first
@@ -73,10 +77,10 @@ __device__ __forceinline__ int group_of(const Batch& b, const Groups& g, int r) 
     int lo = 0, hi = b.G;           // the last group that begins at or in front of r
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (g.off[mid] <= r) lo = mid + 1;
+        if (g.border(mid) <= r) lo = mid + 1;
         else hi = mid;
     }
-    return lo > 0 && r < g.off[lo] ? lo - 1 : -1;
+    return lo > 0 && r < g.border(lo) ? lo - 1 : -1;
 }
 
 // What the arrays say about a request.
@@ -90,12 +94,12 @@ __device__ __forceinline__ Entry entry_of(const Batch& b, const Groups& gs, int 
     Entry x;
     const int span = b.bt_stride * b.page_size;
     if (e < b.G) {
-        const int r0 = clamped(gs.off[e], 0, b.R), r1 = clamped(gs.off[e + 1], r0, b.R);
+        const int r0 = clamped(gs.border(e), 0, b.R), r1 = clamped(gs.border(e + 1), r0, b.R);
         x.table = min(r0, b.R - 1);
         x.first = token_of(b, r0);
         x.tokens = r1 > r0 ? max(token_of(b, r1) - x.first, 0) : 0;
         x.key_lo = 0;
-        x.key_hi = clamped(gs.prefix[e], 0, span);
+        x.key_hi = clamped(gs.shared(e), 0, span);
         x.pos0 = 0x3fffffff;        // every token sees the whole prefix
     } else {
         const int r = e - b.G, g = group_of(b, gs, r);
@@ -103,7 +107,7 @@ __device__ __forceinline__ Entry entry_of(const Batch& b, const Groups& gs, int 
         x.first = raw.first;
         x.tokens = max(raw.end - x.first, 0);
         const int ctx = clamped(raw.ctx, 0, span);
-        x.key_lo = g >= 0 ? clamped(gs.prefix[g], 0, ctx) : 0;
+        x.key_lo = g >= 0 ? clamped(gs.shared(g), 0, ctx) : 0;
         x.key_hi = min(ctx + x.tokens, span);
         x.pos0 = ctx;
     }
@@ -156,11 +160,11 @@ template <int THREADS>
 __device__ __forceinline__ Groups hold_groups(const Batch& b, GroupScratch& s, Raw& raw) {
     const int i = threadIdx.x, r = i * ((b.G + b.R + THREADS - 1) / THREADS) - b.G;
     raw = r >= 0 && r < b.R ? raw_of(b, r) : Raw{0, 0, 0};
-    if (b.G > kGroupsHeld) return Groups{b.group_off, b.prefix_len};
+    if (b.G > kGroupsHeld) return Groups{b.group_off, b.prefix_len, false};
     if (i <= b.G) s.off[i] = ld_step(b.group_off + i);
     if (i >= 32 && i - 32 < b.G) s.prefix[i - 32] = ld_step(b.prefix_len + i - 32);
     __syncthreads();
-    return Groups{s.off, s.prefix};
+    return Groups{s.off, s.prefix, true};
 }
 
 // All threads of the block.  owned[k]: where entry blockIdx.x + k gridDim.x begins, whose tokens this CTA notes.

@@ -143,6 +143,33 @@ def test_the_batch_names_neighbours_that_share():
     assert build(("a", 1), ("c", 1), ("a1", 1)).shared is None      # no neighbours
 
 
+def test_neighbours_that_share_nothing_are_one_run():
+    """Only the runs that share count: a step of many requests has no more groups than a block keeps copies of."""
+    m = CacheManager([CacheNeeds(paged=PagedKVNeeds(1, 16, None))], [None], num_pages=200, page_size=4, max_requests=60,
+                     max_positions=64, dtype=torch.float32, device="cpu")
+    b = BatchBuilder(m, device="cpu", q_tile_sizes=(16,))
+    alone = [f"alone{i}" for i in range(40)]
+    for r in ("a", "b", *alone):
+        m.register(r)
+        grow(m, r, 8)
+    for r, of in (("a1", "a"), ("a2", "a"), ("b1", "b")):
+        m.fork(r, of, 8)
+
+    def runs(*order, portion=()):
+        for r in order:
+            m.reserve(r, 2 if r in portion else 1)
+        s = b.build([StepEntry(r, [0, 0] if r in portion else [0], [0]) for r in order])[0].shared
+        for r in order:
+            m.cancel(r)
+        return s.group_off.tolist(), s.prefix_len.tolist(), s.saved_bits
+
+    assert runs(*alone, "a", "a1", "a2") == ([0, 40, 43], [0, 8], (16).bit_length())
+    assert runs("a", "a1", *alone, "b", "b1") == ([0, 2, 42, 44], [8, 0, 8], (16).bit_length())
+    assert runs("b", "alone0", "a", "b1", "a1", "a2", "alone1") == ([0, 4, 6, 7], [0, 8, 0], (8).bit_length())
+    # portions come first
+    assert runs(*alone, "a", "a1", "b", "b1", portion=("alone3", "b", "b1")) == ([0, 1, 3, 42, 44], [0, 8, 0, 8], (16).bit_length())
+
+
 @pytest.fixture(scope="module")
 def root(tmp_path_factory):
     return str(tmp_path_factory.mktemp("fork"))

@@ -234,3 +234,53 @@ def test_many_requests_with_few_keys_of_their_own(ops, nq, nkv, hd, page):
     case.check(case.call(ops), "bfloat16")
     again = case.call(ops, out=torch.full_like(case.out, 2.0))
     assert torch.equal(again, case.out)
+
+
+@pytest.mark.parametrize("dtype,heads", [(torch.bfloat16, (14, 2, 64)), (torch.float32, (4, 2, 64))])
+def test_borders_of_many_groups_change_between_replays(ops, dtype, heads):
+    """More groups than a block keeps copies of, each call behind others of the same table (so it begins before they have
+    ended), and a graph that is replayed with other borders and prefixes at the same addresses."""
+    nq, nkv, hd = heads
+    cases = []
+    for seed, sizes in ((41, [1, 4, 2, 3, 1]), (42, [3, 1, 1, 5, 1])):        # 80 groups of 176 requests
+        members = [sizes[g % 5] for g in range(80)]
+        cases.append(Case(nq, nkv, hd, 16, [(16 * (g % 7) + seed % 5, ones(*[(5 * g + i) % 29 for i in range(n)]))
+                                            for g, n in enumerate(members)], dtype, seed=seed))
+    a, b = cases
+    assert a.qkv.shape == b.qkv.shape and a.group_off.numel() == b.group_off.numel() == 81
+    assert not torch.equal(a.group_off, b.group_off)
+    width, pages = max(c.table.shape[1] for c in cases), max(c.keys.shape[0] for c in cases)
+    hold = {n: torch.zeros_like(getattr(a, n)) for n in ("qkv", "ctx_len", "prefix_len", "group_off")}
+    hold["table"] = torch.full((a.table.shape[0], width), -1, dtype=torch.int32, device="cuda")
+    hold["keys"] = torch.zeros((pages, *a.keys.shape[1:]), dtype=dtype, device="cuda")
+    hold["values"] = torch.zeros_like(hold["keys"])
+    outs = [torch.empty_like(a.out) for _ in range(4)]
+
+    def load(c):
+        for n in ("qkv", "ctx_len", "prefix_len", "group_off"):
+            hold[n].copy_(getattr(c, n))
+        hold["table"].fill_(-1)
+        hold["table"][:, :c.table.shape[1]] = c.table
+        hold["keys"][:c.keys.shape[0]] = c.keys
+        hold["values"][:c.keys.shape[0]] = c.values
+
+    def calls():
+        for out in outs:
+            ops.shared_prefix_attention(hold["qkv"], hold["keys"], hold["values"], hold["table"], hold["ctx_len"],
+                                        hold["prefix_len"], hold["group_off"], nq, nkv, hd, a.scale, out)
+
+    load(a)
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls()
+    for c in (b, a, b, b, a):
+        load(c)
+        for out in outs:
+            out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(outs[0], sums(c))
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
+    ops.check_errors()

@@ -40,3 +40,17 @@ def test_another_blocks_shared_memory_is_touched_behind_a_cluster_barrier():
             assert "cluster.sync()" in before or ("cluster.barrier_arrive()" in before and "cluster.barrier_wait(" in before), (
                 name, kernel.group(1))
     assert found >= 4
+
+
+def test_a_steps_lengths_are_read_through_l2_before_the_wait():
+    """What a step uploads is read in front of the wait for the kernels before, where only `ld_step` may read it: no entry,
+    group or range of attention over shared prefixes is found by a plain load of the step's arrays."""
+    text = code("shared_prefix.cuh")
+    reads = body(text, "struct Groups")
+    assert re.findall(r"ld_step\((\w+) \+ g\)", reads) == ["off", "prefix"]
+    for name in ("group_of", "raw_of", "token_of", "Entry entry_of", "Groups hold_groups", "Range find_range"):
+        inside = body(text, name + "(")
+        arrays = r"(?:cu_q|ctx_len|prefix_len|group_off|block_table|(?:gs?)\.(?:off|prefix))"
+        assert not re.search(arrays + r"\s*\[", inside), name
+        for use in re.finditer(arrays + r"\s*\+", inside):
+            assert inside[:use.start()].endswith("ld_step(b."), name
