@@ -367,6 +367,7 @@ SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_strid
         return SOMI_ERR_UNSUPPORTED;
     const int per = nq / nkv;
     if (kernel && (dtype != SOMI_BF16 || !somi_shared_attention_tc_takes(nq, nkv, hd, page_size))) return SOMI_ERR_UNSUPPORTED;
+    if (kernel == 1 && !(scale > 0.f)) return SOMI_ERR_UNSUPPORTED;      // (it scales a row's maximum, and hidden scores)
     if (kernel == 2 && static_cast<long long>(T) * per > kFewRows) return SOMI_ERR_UNSUPPORTED;
     const long long span = static_cast<long long>(bt_stride) * page_size;
     const int block_rows = somi_shared_attention_block_rows(kernel);

@@ -727,13 +727,14 @@ class CudaOps:
         if T == 0 or R == 0:
             return
         code = _code(qkv)
-        key = (code, nq, nkv, hd, page_size, self.use_shared_tc, min(T, 17))
+        key = (code, nq, nkv, hd, page_size, self.use_shared_tc, min(T, 17), scale > 0)
         plan = self._shared_plans.get(key)
         if plan is None:
-            # 0 the kernel for any size, 1 the one on tensor cores, 2 that for up to 16 rows a key/value head
+            # 0 the kernel for any size, 1 the one on tensor cores, 2 that for up to 16 rows a key/value head.  (1 takes a row's
+            # maximum before it scales, so it wants a positive scale.)
             kernel = 0
             if code == _BF16 and self.use_shared_tc and self.lib.somi_shared_attention_tc_takes(nq, nkv, hd, page_size):
-                kernel = 2 if T * (nq // nkv) <= 16 else 1
+                kernel = 2 if T * (nq // nkv) <= 16 else 1 if scale > 0 else 0
             plan = self._shared_plans[key] = (kernel, int(self.lib.somi_shared_attention_ctas(hd, kernel)),
                                               int(self.lib.somi_shared_attention_block_rows(kernel)))
         kernel, ctas, block_rows = plan

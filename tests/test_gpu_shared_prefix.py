@@ -284,3 +284,19 @@ def test_borders_of_many_groups_change_between_replays(ops, dtype, heads):
         c.check(outs[0], sums(c))
         assert all(torch.equal(outs[0], o) for o in outs[1:])
     ops.check_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("few", [True, False])
+def test_scales_of_any_sign(ops, dtype, few):
+    """Negative scales with negated queries are the same scores; at 0 all keys weigh the same."""
+    groups = [(160, ones(0, 30) if few else [(0, 5), (37, 1), (9, 70)] + ones(*range(20)))]
+    case = Case(8, 2, 64, 16, groups, dtype, seed=51, scale=0.3)
+    want = case.call(ops).clone()
+    case.check(want, sums(case))
+    case.qkv, case.scale = -case.qkv, -0.3
+    got = case.call(ops, out=torch.full_like(case.out, 7.0))
+    case.scale = 0.3
+    case.check(got, sums(case))
+    flat = Case(8, 2, 64, 16, groups, dtype, seed=52, scale=0.0)
+    flat.check(flat.call(ops), sums(flat))

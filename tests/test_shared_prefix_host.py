@@ -115,3 +115,14 @@ def test_the_rule_of_a_step(ops):
     assert not pays(15 * 176, 0, 16, 16 * 64) and not pays(15 * 4096, 0, 16, 16 * 200)
     ops.use_shared_prefix = False
     assert not pays(63 * 2048, 64)
+
+
+def test_the_kernel_that_scales_a_maximum_takes_positive_scales_only(ops):
+    ops.lib.somi_shared_attention_tc_takes = lambda nq, nkv, hd, page: 1
+    many = {n: torch.zeros(40, 5, dtype=torch.int32) if n == "block_table" else torch.zeros(40, dtype=torch.int32)
+            for n in ("block_table", "ctx_len")}
+    many.update({n: torch.zeros(40, 256).bfloat16() for n in ("qkv", "out")})
+    many.update({n: torch.zeros(9, 2, 16, 64).bfloat16() for n in ("kcache", "vcache")})
+    for scale, kernel in ((0.5, 1), (-0.5, 0), (0.5, 1), (0.0, 0), (float("nan"), 0)):
+        ops.shared_prefix_attention(**arguments(scale=scale, **many))
+        assert ops.calls[-1][20] == kernel
