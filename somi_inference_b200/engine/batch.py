@@ -16,7 +16,7 @@ find a contiguous range; `logit_rows` keeps the caller's order.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import numpy as np
 import torch
@@ -40,6 +40,20 @@ class GroupBatch:
     width: int
 
 
+# A portion of a prompt reads far more than it brings behind this many cached positions, and four times its own; with more tokens
+# than the second it fills tiles well by itself (`CudaOps.shared_prefix_pays` says what was measured).
+DEEP_PORTION = 256
+LONG_PORTION = 1024
+
+
+class PortionFacts(NamedTuple):
+    """What a step's multi-token requests have to do with what it shares."""
+
+    saved_bits: int             # as above, of the runs that have such a request among their members
+    deep: bool                  # one of them continues from DEEP_PORTION cached positions or more, and four times its tokens
+    long: bool                  # one of them has more than LONG_PORTION tokens
+
+
 @dataclass
 class SharedPrefixes:
     """Neighbouring requests of the batch that share their first positions (forks, `CacheManager.fork`)."""
@@ -48,6 +62,7 @@ class SharedPrefixes:
     group_off: torch.Tensor         # int32 [G + 1] group g is requests [group_off[g], group_off[g + 1])
     # bits of the number of positions that need not be read again: sum of prefix_len * (members - 1)
     saved_bits: int
+    portions: PortionFacts | None = None    # None: single tokens only
 
 
 @dataclass
@@ -123,12 +138,13 @@ class BatchBuilder:
         self._capacity = capacity
         self.generation = getattr(self, "generation", 0) + 1    # device addresses changed
 
-    def _shared_runs(self, requests) -> tuple[list[int], list[int], int] | None:
-        """(borders of the runs of neighbours that share, what each shares, bits of what that saves), or None.
+    def _shared_runs(self, requests, portions: int = 0) -> tuple[list[int], list[int], int, int] | None:
+        """(borders of the runs of neighbours that share, what each shares, bits of what that saves, bits of what the runs
+        save that hold one of the first `portions` requests), or None.
         Neighbours that share nothing are one run of 0 positions: the kernel finds few runs faster."""
         if not self.cache.any_family:
             return None
-        off, shared, last, saved = [0], [], None, 0
+        off, shared, last, saved, by_portions = [0], [], None, 0, 0
         for j, r in enumerate(requests):
             family, n = self.cache.family(r)
             if j and (family != last or not family):
@@ -144,6 +160,7 @@ class BatchBuilder:
             members = off[g + 1] - off[g]
             n = n if members > 1 else 0
             saved += n * (members - 1)
+            by_portions += n * (members - 1) if off[g] < portions else 0
             if prefixes and prefixes[-1] == n == 0:
                 ends[-1] = off[g + 1]
             else:
@@ -151,7 +168,7 @@ class BatchBuilder:
                 prefixes.append(n)
         if not saved:
             return None
-        return ends, prefixes, saved.bit_length()
+        return ends, prefixes, saved.bit_length(), by_portions.bit_length()
 
     @property
     def h2d_bytes_last(self) -> int:
@@ -251,8 +268,11 @@ class BatchBuilder:
         arrays += [tiles_np[bm].reshape(-1) for bm in self.q_tile_sizes]
         for gi in range(len(tables)):
             arrays += [tables[gi].reshape(-1), slot_maps[gi]]
-        runs = self._shared_runs([entries[i].request for i in order])
+        runs = self._shared_runs([entries[i].request for i in order], n_prefill)
+        facts = None
         if runs:
+            deep = ctx[:n_prefill] >= np.maximum(DEEP_PORTION, 4 * q_lens[:n_prefill])
+            facts = PortionFacts(runs[3], bool(deep.any()), bool(q_lens.max() > LONG_PORTION))
             sizes += [len(runs[0]), len(runs[1])]
             arrays += runs[:2]
         offsets, total = self._upload(sizes, arrays)
@@ -274,8 +294,8 @@ class BatchBuilder:
             state_slot=dv(5), logit_rows=dv(6), tiles=tiles, groups=groups,
             host=HostBatch(cu_q=cu_q, ctx_len=ctx, state_slot=slots,
                            requests=[entries[i].request for i in order]),
-            layout_key=tuple(sizes) + (n_prefill, n_prefill_tokens) + (runs[2:] if runs else ()),
-            shared=SharedPrefixes(dv(at - 1), dv(at - 2), runs[2]) if runs else None,
+            layout_key=tuple(sizes) + (n_prefill, n_prefill_tokens) + ((runs[2], facts) if runs else ()),
+            shared=SharedPrefixes(dv(at - 1), dv(at - 2), runs[2], facts) if runs else None,
         )
         return batch, order
 
@@ -358,7 +378,7 @@ class BatchBuilder:
             logit_rows=fixed[6], tiles=tiles, groups=groups,
             host=HostBatch(cu_q=np.arange(R + 1, dtype=np.int64), ctx_len=pos_np,
                            state_slot=slots_np, requests=reqs),
-            layout_key=tuple(sizes) + (0, 0) + (runs[2:] if runs else ()),
+            layout_key=tuple(sizes) + (0, 0) + (runs[2:3] if runs else ()),
             shared=SharedPrefixes(*shared, runs[2]) if runs else None)
         return batch, list(range(R))
 

@@ -422,7 +422,7 @@ class CudaOps:
             if gate is not None or vd % 2:
                 raise KernelError("turned outputs come in pairs and without a gate")
         shared = getattr(batch, "shared", None)
-        if shared is not None and self.shared_prefix_pays(shared.saved_bits, batch, nq, nkv, hd, qkv, page_size) and vd == hd and not (
+        if shared is not None and self.shared_prefix_pays(shared.saved_bits, batch, nq, nkv, hd, qkv, page_size, shared.portions) and vd == hd and not (
                 win or chunk or cap or sinks is not None or turn is not None or gate is not None):
             self.shared_prefix_attention(qkv, kcache, vcache, group.block_table, batch.ctx_len, shared.prefix_len,
                                          shared.group_off, nq, nkv, hd, scale, out,
@@ -757,27 +757,51 @@ class CudaOps:
     # (2^23) 15.0 and 17.2, 8 behind 8,192 (2^24) 25.8 and 17.8, 64 behind 2,048 (2^25) 44.8 and 25.3; what every request
     # has read once lies in L2, and a step takes the longer way of parts, products of whole tiles and a merge.
     SHARED_PREFIX_VALUES = 1 << 25
-    # ... and positions a request of the step, since each has a piece of its own, whose chain is longer than a split of the usual
-    # kernel: beside 16 behind 4,096, 24 requests of 4,000 that share nothing 63.5 us and 52.2, 64 of 500 36.1 and 45.5
+    # ... and positions a request of the step, since each has a piece of its own, whose chain is longer than a split of the
+    # usual kernel: beside 16 behind 4,096, 24 requests of 4,000 that share nothing 63.6 us and 50.6, 64 of 500 35.7 and 32.0.
+    # Where a position is fewer than 512 elements, more of them: 14 heads of 64 over 2, beside 40 behind 4,096, 108 of 60
+    # 20.3 us and 22.3, of 4,000 62.8 and 74.6
     SHARED_PREFIX_POSITIONS = 1024
     # Short portions fill tiles of their own badly: 4 portions of 16 behind 512 (2^19) 16.6 us and 16.6, 2 behind 2,048
     # (2^20) 40.9 and 19.1, 64 of 2 behind 64 (2^20) 72.5 and 19.2.  Longer ones gain only behind much longer prefixes:
     # of 64, 16 behind 176 33.8 and 48.6, 8 behind 1,024 40.3 and 38.4, 16 behind 4,096 229.7 and 99.2; of 128, 16 behind
     # 4,096 241 and 179; of 200 285 and 283.
     SHARED_PREFIX_VALUES_PORTIONS = 1 << 20
+    # Beside single tokens that share nothing (28 heads of 128 over 4; 40 over 8 in brackets): 2 of 16 behind 1,024 with 64 of
+    # 500 42.0 us and 30.9 (56.0 and 45.6), with 200 of 300 62.1 and 58.7 (91.0 and 94.1); 4 of 2 behind 512 with 200 of 60
+    # 35.6 and 40.2 (53.2 and 67.5).  So they, too, want some positions a request of the step.
+    SHARED_PREFIX_POSITIONS_PORTIONS = 16
+    # A short portion behind many cached positions of its own gains less, unless there are very many: 16 at 300 beside 8 single
+    # tokens behind 2,048 20.8 us and 15.2 (26.3 and 17.5), and 100 of 60 that share nothing 29.3 and 29.3 (41.8 and 45.9).
+    SHARED_PREFIX_POSITIONS_DEEP = 256
 
-    def shared_prefix_pays(self, saved_bits: int, batch, nq: int, nkv: int, hd: int, qkv, page_size: int) -> bool:
+    def shared_prefix_pays(self, saved_bits: int, batch, nq: int, nkv: int, hd: int, qkv, page_size: int, portions=None) -> bool:
         """Whether a step of bfloat16 goes to `shared_prefix_attention`: where the positions that it does not read again
-        (a number of `saved_bits` bits) are worth more than its longer way."""
+        (a number of `saved_bits` bits) are worth more than its longer way.  `portions` (`PortionFacts`): what the step's
+        multi-token requests have to do with them (None: all of them share).
+
+        Where such requests share, or lie behind many cached positions, it is they who gain.  Where they do neither, the
+        single tokens decide as if they were alone: with a new prompt of 16, 2 behind 1,024 10.2 us and 14.0, 8 behind 512 10.9 and
+        12.8, 16 behind 4,096 32.1 and 19.0.  One portion of more than 1,024 tokens takes what short ones gain: 64 of 2 behind
+        64 beside 900 at 8,000 177 us and 148, beside 1,900 279 and 311."""
         if not self.use_shared_prefix or qkv.dtype != torch.bfloat16 or qkv.shape[1] % 8 or batch.num_requests > 4096:
             return False
-        portions, values = batch.num_prefill_requests, nkv * hd << saved_bits
-        if portions == 0:
-            pays = values >= self.SHARED_PREFIX_VALUES and 1 << saved_bits >= self.SHARED_PREFIX_POSITIONS * batch.num_requests
-        else:
-            mean = batch.num_prefill_tokens / portions
-            pays = values >= self.SHARED_PREFIX_VALUES_PORTIONS and (
-                mean <= 32 or (mean <= 128 and 1 << saved_bits >= 32 * batch.num_tokens))
+        requests, elements = batch.num_requests, nkv * hd
+
+        def saves(bits, values, positions):
+            return bits > 0 and elements << bits >= values and 1 << bits >= positions * requests
+
+        pays = saves(saved_bits, self.SHARED_PREFIX_VALUES, self.SHARED_PREFIX_POSITIONS * max(1, 512 / elements))
+        if batch.num_prefill_requests:
+            values, few = self.SHARED_PREFIX_VALUES_PORTIONS, self.SHARED_PREFIX_POSITIONS_PORTIONS
+            if portions is None:
+                pays = pays or saves(saved_bits, values, few)
+            else:
+                pays = not portions.long and (
+                    pays or saves(portions.saved_bits, values, few)
+                    or (portions.deep and saves(saved_bits, values, self.SHARED_PREFIX_POSITIONS_DEEP)))
+            mean = batch.num_prefill_tokens / batch.num_prefill_requests
+            pays = pays and (mean <= 32 or (mean <= 128 and 1 << saved_bits >= 32 * batch.num_tokens))
         return pays and bool(self.lib.somi_shared_attention_tc_takes(nq, nkv, hd, page_size))
 
     def two_map_attention(self, qkv, kcache, vcache, batch, group, nq, nkv, d, vd, scale, window, keep,

@@ -170,6 +170,41 @@ def test_neighbours_that_share_nothing_are_one_run():
     assert runs(*alone, "a", "a1", "b", "b1", portion=("alone3", "b", "b1")) == ([0, 1, 3, 42, 44], [0, 8, 0, 8], (16).bit_length())
 
 
+def test_a_batch_says_what_its_portions_share():
+    """What decides which kernels a step launches is part of its layout."""
+    m = CacheManager([CacheNeeds(paged=PagedKVNeeds(1, 16, None))], [None], num_pages=2000, page_size=4, max_requests=20,
+                     max_positions=4000, dtype=torch.float32, device="cpu")
+    b = BatchBuilder(m, device="cpu", q_tile_sizes=(16,))
+    for r, n in (("a", 300), ("b", 8), ("new", 0), ("deep", 256), ("deeper", 1200)):
+        m.register(r)
+        if n:
+            grow(m, r, n)
+    for r, of, n in (("a1", "a", 300), ("a2", "a", 300), ("b1", "b", 8), ("b2", "b", 8)):
+        m.fork(r, of, n)
+
+    def build(**entries):
+        for r, n in entries.items():
+            m.reserve(r, n)
+        batch = b.build([StepEntry(r, [0] * n, [0]) for r, n in entries.items()])[0]
+        for r in entries:
+            m.cancel(r)
+        return batch
+
+    def facts(**entries):
+        return build(**entries).shared.portions
+
+    assert facts(a=1, a1=1) is None                               # single tokens only
+    assert facts(a=1, a1=1, new=3) == (0, False, False)
+    assert facts(b=2, b1=1, a=1, a1=1) == ((8).bit_length(), False, False)      # the run of portions goes on among single tokens
+    assert facts(b=1, b1=1, a=2, a1=3) == ((300).bit_length(), True, False)
+    assert facts(a=1, a1=1, deep=64) == (0, True, False) and facts(a=1, a1=1, deep=65) == (0, False, False)
+    assert facts(a=1, a1=1, b=1, b1=1, new=1024) == (0, False, False) and facts(a=1, a1=1, new=1025) == (0, False, True)
+    assert facts(a=1, a1=1, deeper=300) == (0, True, False)
+    # equal sizes, other facts: other layouts
+    one, two = build(a=1, a1=1, deep=64, new=66), build(a=1, a1=1, deep=66, new=64)
+    assert one.layout_key != two.layout_key and one.layout_key[:-1] == two.layout_key[:-1]
+
+
 @pytest.fixture(scope="module")
 def root(tmp_path_factory):
     return str(tmp_path_factory.mktemp("fork"))

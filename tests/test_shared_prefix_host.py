@@ -117,6 +117,41 @@ def test_the_rule_of_a_step(ops):
     assert not pays(63 * 2048, 64)
 
 
+def test_the_rule_of_a_step_of_portions_and_single_tokens(ops):
+    """Portions that share nothing leave the decision to the single tokens, unless they lie behind many positions of their
+    own; requests that share nothing, and long portions, count against what is saved."""
+    from types import SimpleNamespace
+    from somi_inference_b200.engine.batch import PortionFacts
+    ops.use_shared_prefix = True
+    ops.lib.somi_shared_attention_tc_takes = lambda nq, nkv, hd, page: 1
+
+    def pays(saved, portions, singles=0, by_portions=0, deep=False, long=False, heads=(28, 4, 128)):
+        """`portions`: their tokens."""
+        nq, nkv, hd = heads
+        batch = SimpleNamespace(num_requests=singles + len(portions), num_prefill_requests=len(portions),
+                                num_prefill_tokens=sum(portions), num_tokens=singles + sum(portions))
+        facts = PortionFacts(by_portions.bit_length(), deep, long)
+        return ops.shared_prefix_pays(saved.bit_length(), batch, nq, nkv, hd, torch.zeros(1, (nq + 2 * nkv) * hd).bfloat16(), 16, facts)
+
+    # single tokens that are refused alone are refused beside a prompt that shares nothing
+    assert not pays(7 * 2048, [16], singles=8) and not pays(7 * 512, [2], singles=8) and not pays(1024, [16], singles=2)
+    assert pays(7 * 2048, [16], singles=8, deep=True) and not pays(7 * 2048, [16], singles=108, deep=True)
+    # ... and those that are taken alone are taken, if it is short
+    assert pays(15 * 4096, [16], singles=16) and not pays(15 * 4096, [300], singles=16) and not pays(15 * 4096, [16], singles=80)
+    # portions that share
+    assert pays(1024, [16, 16], by_portions=1024) and pays(1024, [16, 16], singles=64, by_portions=1024)
+    assert not pays(1024, [16, 16], singles=200, by_portions=1024) and not pays(3 * 512, [2] * 4, singles=200, by_portions=3 * 512)
+    # what portions save among themselves is too little, and the single tokens decide
+    assert not pays(7 * 2048 + 16, [2, 2], singles=8, by_portions=16)
+    # thirty of 2 beside one of 900, and beside one of 1,025
+    assert pays(29 * 2048, [2] * 30 + [900], by_portions=29 * 2048)
+    assert not pays(29 * 2048, [2] * 60 + [1025], by_portions=29 * 2048, long=True)
+    # few elements a position: more positions a request
+    small = (14, 2, 64)
+    assert pays(63 * 8192, [], singles=64, heads=small) and not pays(39 * 4096, [], singles=148, heads=small)
+    assert pays(39 * 4096, [], singles=148) and not pays(0, [16, 16], singles=4)
+
+
 def test_the_kernel_that_scales_a_maximum_takes_positive_scales_only(ops):
     ops.lib.somi_shared_attention_tc_takes = lambda nq, nkv, hd, page: 1
     many = {n: torch.zeros(40, 5, dtype=torch.int32) if n == "block_table" else torch.zeros(40, dtype=torch.int32)
