@@ -10,7 +10,8 @@
 // on the order of summation nor on float32's rounding: a weight is computed in float64 (2^r by its Taylor
 // series, relative error 3e-16) and held as an integer multiple of 2^-44, and sums of integers are exact.
 // (Fewer than 2^20 weights of at most 2^44 stay below 2^64.)  So the result is the same bits whatever the launch
-// looks like, and differs from real arithmetic only where a border lies within about 1e-11 of the number.
+// looks like, and differs from real arithmetic only where a border lies within n 2^-45 of the number, n the tokens with a
+// weight, in units of the largest weight: 4e-9 for 152,064 tokens whose roundings all have one sign.
 //
 // A cluster of CTAs shares a row; each holds its slice in shared memory, read from HBM once, as a bulk copy where
 // the row is aligned.  A warp owns a contiguous segment of it.  All three cuts keep a beginning of one order, so a
@@ -51,6 +52,7 @@ constexpr int kListed = 2048;                // survivors that one CTA takes
 constexpr int kBinListed = 1024;             // tokens of top-p's bin that one CTA takes
 constexpr int kCounted = 2 * 16 * 128;       // values of 16-bit logits that are counted: signs, exponents (2^-8 to 2^8), mantissas
 constexpr unsigned kCountedFrom = 119u << 7;
+constexpr int kMostSlice = 192 * 1024;       // bytes of a slice beside the static shared memory
 constexpr int kFraction = 44;                // a weight is an integer multiple of 2^-44
 typedef unsigned long long u64;
 
@@ -931,6 +933,12 @@ draw_kernel(const T* __restrict__ logits, long long stride, int V, int seg, Sett
     // (nobody reads another CTA's memory behind the last sum: all may leave)
 }
 
+// Tokens of a row, at most: the slices of the largest cluster, and sums of weights below 2^64.
+template <typename T>
+constexpr int most_tokens() {
+    return std::min(kMaxCluster * kMostSlice / static_cast<int>(sizeof(T)), (1 << 20) - 1);
+}
+
 template <typename T>
 int launch_draw(const void* logits, long long stride, int rows, int V, const Settings& set, const float* uniform, int draws,
                 int* out, float* prob, cudaStream_t stream) {
@@ -939,13 +947,12 @@ int launch_draw(const void* logits, long long stride, int rows, int V, const Set
     // (16 CTAs a row while the rows' clusters find room beside each other: 152,064 logits with top-k, top-p and min-p, 1 row 11.7 us,
     // with 8 13.1; 12 rows 14.4 and 15.8; 16 rows 20.5 and 16.5)
     while (ranks < (rows <= 12 ? kMaxCluster : 8) && V > ranks * 4096 && !(rows * ranks >= 256 && bytes_of(ranks) <= 78 * 1024)) ranks *= 2;
-    const int most = 192 * 1024;             // bytes of a slice beside the static shared memory
     const auto segment = [&](int n) { return ((V + n * kWarps - 1) / (n * kWarps) + 7) / 8 * 8; };
-    while (ranks < kMaxCluster && static_cast<long long>(segment(ranks)) * kWarps * sizeof(T) > most) ranks *= 2;
+    while (ranks < kMaxCluster && static_cast<long long>(segment(ranks)) * kWarps * sizeof(T) > kMostSlice) ranks *= 2;
     const int seg = segment(ranks);
     const long long bytes = std::max(static_cast<long long>(seg) * kWarps * static_cast<long long>(sizeof(T)), 24ll * kListed);
-    if (bytes > most || V >= 1 << 20 || static_cast<long long>(rows) * ranks > 0x7fffffffll) return SOMI_ERR_UNSUPPORTED;
-    allow_smem<draw_kernel<T>>(most);
+    if (V > most_tokens<T>() || bytes > kMostSlice || static_cast<long long>(rows) * ranks > 0x7fffffffll) return SOMI_ERR_UNSUPPORTED;
+    allow_smem<draw_kernel<T>>(kMostSlice);
     if (ranks > 8 && cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
         return SOMI_ERR_UNSUPPORTED;
     return launch_pdl_cluster(draw_kernel<T>, dim3(static_cast<unsigned>(rows) * ranks), dim3(kThreads), static_cast<size_t>(bytes),
@@ -963,6 +970,11 @@ SOMI_API int somi_draw_error() {
     if (cudaMemcpyFromSymbol(&v, draw::g_draw_error, sizeof(int)) != cudaSuccess) return -1;
     if (v) cudaMemcpyToSymbol(draw::g_draw_error, &zero, sizeof(int));
     return v;
+}
+
+// The largest vocabulary of a type, 0 where it is not taken.
+SOMI_API int somi_draw_max_vocabulary(int dtype) {
+    return dtype == SOMI_F32 ? draw::most_tokens<float>() : dtype == SOMI_BF16 ? draw::most_tokens<__nv_bfloat16>() : 0;
 }
 
 // logits [rows, V] (rows `stride` elements apart), uniform, out and prob (or null) [rows, draws]; temperature, top_k,

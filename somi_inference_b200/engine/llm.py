@@ -115,6 +115,10 @@ class LLM:
                      sampling_params: SamplingParams | None = None,
                      ignore_eos: bool = False) -> Request:
         sp = sampling_params or SamplingParams()
+        most = getattr(self.engine.ops, "DRAW_MAX_VOCABULARY", {}).get(torch.float32)
+        if sp.min_p > 0.0 and sp.temperature > 0.0 and most and self.engine.spec.vocab_size > most:
+            raise ValueError(f"min_p is sampled from vocabularies of up to {most} tokens; the model has "
+                             f"{self.engine.spec.vocab_size}")
         seed = sp.seed if sp.seed is not None else random.getrandbits(63)
         req = Request(self._next_request_id, list(prompt_tokens), max_new_tokens, sp,
                       ignore_eos=ignore_eos, seed=int(seed))

@@ -2282,11 +2282,14 @@ class CudaOps:
         if trace.active():
             trace.note("sample", logits.numel() * 4)
 
+    # tokens of a row that `draw_tokens` takes (its clusters' shared memory; sums of weights below 2^64)
+    DRAW_MAX_VOCABULARY = {torch.float32: 786432, torch.bfloat16: (1 << 20) - 1}
+
     def draw_tokens(self, logits, uniform, temperature, top_k, top_p, min_p, out, prob=None, penalty=None,
                     hist_off=None, hist_tok=None) -> None:
         """Tokens drawn from rows of logits with the caller's random numbers.
 
-        `logits` [rows, V] float32 or bfloat16 (rows may lie further apart); `uniform` float32 [rows] or
+        `logits` [rows, V] float32 (V up to 786,432) or bfloat16 (up to 1,048,575; rows may lie further apart); `uniform` float32 [rows] or
         [rows, n], numbers in [0, 1): n draws of a row; `out` int32 and `prob` float32 (or None) of
         the same shape: the tokens, and the probability that each was drawn with.  Per row: `temperature`
         (<= 0: the lowest index of the maximum), `top_k` int32 (<= 0 or >= V: off), `top_p` (>= 1: off), `min_p` (<= 0: off).
@@ -2328,6 +2331,9 @@ class CudaOps:
             raise KernelError("draw_tokens takes uniform, out and prob of one shape, [rows] or [rows, draws], and settings [rows]")
         draws = shape[1] if len(shape) == 2 else 1
         code = _code(logits)
+        if V > self.DRAW_MAX_VOCABULARY.get(logits.dtype, V):
+            raise KernelError(f"draw_tokens takes vocabularies of up to {self.DRAW_MAX_VOCABULARY[logits.dtype]} tokens with logits of "
+                              f"{logits.dtype}, not {V}")
         if rows == 0 or draws == 0:
             return
         rc = self._draw(logits.data_ptr(), code, logits.stride(0), rows, V, uniform.data_ptr(), draws, temperature.data_ptr(),

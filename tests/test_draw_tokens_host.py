@@ -77,6 +77,34 @@ def test_refusals(ops, changed):
     assert not ops.calls and ops.launches == 0
 
 
+@pytest.mark.parametrize("dtype,most", [(torch.float32, 786432), (torch.bfloat16, 2 ** 20 - 1)])
+def test_a_vocabulary_that_is_too_large_is_named(ops, dtype, most):
+    one = {n: torch.ones(1) for n in ("uniform", "temperature", "top_p", "min_p")}
+    one.update(top_k=torch.zeros(1, dtype=torch.int32), out=torch.zeros(1, dtype=torch.int32))
+    ops.draw_tokens(**arguments(logits=torch.zeros(1, most, dtype=dtype), **one))
+    assert len(ops.calls) == 1
+    with pytest.raises(KernelError, match=str(most)):
+        ops.draw_tokens(**arguments(logits=torch.zeros(1, most + 1, dtype=dtype), **one))
+    assert len(ops.calls) == 1
+
+
+def test_a_request_with_min_p_and_too_large_a_vocabulary_is_refused_before_it_runs():
+    from types import SimpleNamespace
+    from somi_inference_b200 import LLM, SamplingParams
+    llm = LLM.__new__(LLM)
+    llm._next_request_id = 0
+    for size, refused in ((786432, False), (786433, True)):
+        llm.engine = SimpleNamespace(ops=SimpleNamespace(DRAW_MAX_VOCABULARY=cuda.CudaOps.DRAW_MAX_VOCABULARY),
+                                     spec=SimpleNamespace(vocab_size=size))
+        for sp in (SamplingParams(), SamplingParams(min_p=0.5, temperature=0.0)):
+            assert llm.make_request([1], max_new_tokens=1, sampling_params=sp).sampling_params is sp
+        if refused:
+            with pytest.raises(ValueError, match="786432"):
+                llm.make_request([1], max_new_tokens=1, sampling_params=SamplingParams(min_p=0.5))
+        else:
+            llm.make_request([1], max_new_tokens=1, sampling_params=SamplingParams(min_p=0.5))
+
+
 def test_a_tensor_of_the_host_or_another_device_is_refused(ops):
     a = arguments()
     a["top_p"] = torch.ones(3)

@@ -289,3 +289,22 @@ def test_counted_values_of_16_bits(ops):
     for p in (0.3, 0.97):
         check(ops, x, [((1.0, 0.6, 3.0)[r % 3], -1, p, 0.0 if r % 5 else 1e-4) for r in range(17)], u)
     ops.check_errors()
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.bfloat16, 1)])
+def test_the_largest_vocabulary(ops, dtype, code):
+    from somi_inference_b200.ops import KernelError
+    V = ops.lib.somi_draw_max_vocabulary(code)
+    assert V == ops.DRAW_MAX_VOCABULARY[dtype]
+    g = torch.Generator().manual_seed(50)
+    x = (torch.randn(4, V, generator=g) * 3).to(dtype)
+    x[2:] = (x[2:].float() * 0.2).to(dtype)
+    u = torch.rand(4, 5, generator=g)
+    u[:, 0], u[:, 1] = 0.0, 1.0 - 2.0 ** -24
+    check(ops, x, [(1.0, -1, 1.0, 0.0), (0.8, 40, 0.9, 0.05), (1.0, -1, 0.9, 0.0), (1.0, -1, 1.0, 0.01)], u)
+    one = torch.ones(1, device="cuda")
+    out = torch.full((1,), -5, dtype=torch.int32, device="cuda")
+    with pytest.raises(KernelError, match="vocabular"):
+        ops.draw_tokens(torch.zeros(1, V + 1, dtype=dtype, device="cuda"), 0 * one, one, out, one, one, out)
+    assert out.item() == -5
+    ops.check_errors()
