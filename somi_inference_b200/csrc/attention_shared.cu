@@ -185,6 +185,83 @@ shared_attention_kernel(const Batch b, const T* __restrict__ q, long long q_stri
     write_notes<kThreads>(b, groups, owned, range.total, notes, header, tid);
 }
 
+// What a row that is not finite is computed again from.  `q` null: never.
+template <typename T>
+struct Source {
+    const T *q, *keys, *values;
+    long long q_stride;
+    float scale_log2e;
+};
+
+// A row by itself, over the keys that it sees and nothing else; by one warp, four columns a lane (head sizes to 128).  The
+// tensor-core kernels multiply a value that a row does not see by a probability of 0, and where that value is infinite or not a
+// number the row is lost.  Only a later token of the row's own portion can do that, so nothing is computed where no such token
+// has such a value.  (Few registers rather than many loads in flight: behind 20,000 positions a row takes 20 ms, but the merge keeps
+// its eight blocks an SM, without which 24 portions took 168 us for 163.)
+template <typename T>
+__device__ __noinline__ void row_alone(const Batch& b, const Source<T>& from, int d, int t, int h, T* out) {
+    const int lane = threadIdx.x & 31, c = lane * 4, kvh = h / b.per;
+    int r = 0;
+    for (int hi = b.R - 1; r < hi;) {                // the last request that begins at or in front of t
+        const int mid = (r + hi + 1) >> 1;
+        if (b.cu_q[mid] <= t) r = mid;
+        else hi = mid - 1;
+    }
+    const int span = b.bt_stride * b.page_size, ctx = clamped(b.ctx_len[r], 0, span);
+    const int pos = min(ctx + t - b.cu_q[r], span - 1), end = min(ctx + b.cu_q[r + 1] - b.cu_q[r], span);
+    const int* table = b.block_table + static_cast<size_t>(r) * b.bt_stride;
+    auto row_of = [&](const T* store, int key) {
+        const int page = table[key / b.page_size];
+        F4 v{{0.f, 0.f, 0.f, 0.f}};
+        if (c < d && static_cast<unsigned>(page) < static_cast<unsigned>(b.num_pages))
+            v = load4(store + ((static_cast<size_t>(page) * b.nkv + kvh) * b.page_size + key % b.page_size) * d + c);
+        return v;
+    };
+    bool lost = false;
+    for (int key = pos + 1; key < end; ++key) {
+        const F4 v = row_of(from.values, key);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lost = lost || !isfinite(v.v[e]);
+    }
+    if (!__any_sync(0xffffffffu, lost)) return;
+    F4 q{{0.f, 0.f, 0.f, 0.f}}, o = q;
+    if (c < d) q = load4(from.q + t * from.q_stride + static_cast<size_t>(h) * d + c);
+    float m = -INFINITY, l = 0.f;
+    constexpr int AT_ONCE = 2;
+    for (int k0 = 0; k0 <= pos; k0 += AT_ONCE) {
+        float s[AT_ONCE], top = m;
+        F4 v[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const F4 k = row_of(from.keys, min(k0 + i, pos));
+            v[i] = row_of(from.values, min(k0 + i, pos));
+            s[i] = fmaf(q.v[3], k.v[3], fmaf(q.v[2], k.v[2], fmaf(q.v[1], k.v[1], q.v[0] * k.v[0])));
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            s[i] = k0 + i <= pos ? warp_sum(s[i]) * from.scale_log2e : -INFINITY;
+            top = fmaxf(top, s[i]);
+        }
+        const float ref = top == -INFINITY ? 0.f : top, keep = exp2f(m - ref);
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o.v[e] *= keep;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            if (k0 + i > pos) continue;
+            const float w = exp2f(s[i] - ref);
+            l += w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.v[e] = fmaf(w, v[i].v[e], o.v[e]);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.v[e] *= inv;
+    if (c < d) store4(out + (static_cast<size_t>(t) * b.nq + h) * d + c, o);
+}
+
 constexpr int kFewRowsOut = 4 * 148;     // four blocks an SM
 
 // SPLIT warps per (token, head), a block of WARPS.  A lane finds out where a part lies and loads its maximum and sum, for
@@ -192,8 +269,8 @@ constexpr int kFewRowsOut = 4 * 148;     // four blocks an SM
 // warps, whose sums are joined in shared memory.
 template <typename T, int WARPS, int SPLIT>
 __global__ void __launch_bounds__(WARPS * 32)
-shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const unsigned* __restrict__ header, Parts parts,
-                    int ctas, T* __restrict__ out) {
+shared_merge_kernel(const __grid_constant__ Batch b, int d, const Note* __restrict__ notes, const unsigned* __restrict__ header, Parts parts,
+                    int ctas, const __grid_constant__ Source<T> from, T* __restrict__ out) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31;
@@ -299,24 +376,32 @@ shared_merge_kernel(const Batch b, int d, const Note* __restrict__ notes, const 
             sum = fmaf(state[w].y, f[w], sum);
         }
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        bool lost = false;
         for (int col = threadIdx.x; col < d; col += WARPS * 32) {
             float v = 0.f;
 #pragma unroll
             for (int w = 0; w < SPLIT; ++w) v = fmaf(rows[w][col], f[w], v);
             out[row * d + col] = from_float<T>(v * inv);
+            lost = lost || !isfinite(v * inv);
         }
+        if (from.q && __syncthreads_or(lost) && threadIdx.x < 32) row_alone(b, from, d, t, h, out);
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
+    bool lost = false;
 #pragma unroll
     for (int c = 0; c < COLS; ++c) {
         const int col = (c * 32 + lane) * 4;
         if (col < d) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[c].v[e] *= inv;
+            for (int e = 0; e < 4; ++e) {
+                o[c].v[e] *= inv;
+                lost = lost || !isfinite(o[c].v[e]);
+            }
             store4(out + row * d + col, o[c]);
         }
     }
+    if (from.q && __any_sync(0xffffffffu, lost)) row_alone(b, from, d, t, h, out);
 }
 
 template <typename T, int HD>
@@ -396,15 +481,18 @@ SOMI_API int somi_shared_attention(const void* qkv, int dtype, long long q_strid
             : hd <= 128   ? launch_shared<E, 128>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream)
                           : launch_shared<E, 256>(b, qkv, q_stride, keys, values, hd, scale, notes, header, parts, ctas, stream);
         if (rc) return rc;
+        // (the kernel for any size keeps out what a row does not see, and a single token has no later ones)
+        const Source<E> from{kernel && cu_q ? static_cast<const E*>(qkv) : nullptr, static_cast<const E*>(keys),
+                             static_cast<const E*>(values), q_stride, scale * 1.4426950408889634f};
         const long long out_rows = static_cast<long long>(T) * nq;
         // Few rows have their keys in many CTAs.  One warp a row against eight: 2 requests behind 8,192 positions 32.4 us and
         // 12.5 (14 heads of 64), 8 behind 2,048 14.5 and 13.5 (28 of 128), 32 behind 4,096 19.4 and 16.4 (448 rows), but 896 rows
         // 22.8 and 25.1.  Up to 8 steps of 64 keys there is nothing to divide (2 behind 176: 7.0 and 7.3).
         if (out_rows <= kFewRowsOut && span > 512)
             return launch_pdl(shared_merge_kernel<E, 8, 8>, dim3(static_cast<unsigned>(out_rows)), dim3(256), 0, stream, b, hd, notes,
-                              header, parts, ctas, static_cast<E*>(out));
+                              header, parts, ctas, from, static_cast<E*>(out));
         return launch_pdl(shared_merge_kernel<E, 4, 1>, dim3(static_cast<unsigned>((out_rows + 3) / 4)), dim3(128), 0, stream, b, hd,
-                          notes, header, parts, ctas, static_cast<E*>(out));
+                          notes, header, parts, ctas, from, static_cast<E*>(out));
     };
     return dtype == SOMI_F32 ? launch(float{}) : dtype == SOMI_BF16 ? launch(__nv_bfloat16{}) : SOMI_ERR_UNSUPPORTED;
 }

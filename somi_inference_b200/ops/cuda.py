@@ -694,8 +694,9 @@ class CudaOps:
         numbers of requests, groups and tokens), and before the kernel in front has ended where that is one of this
         table's: none of these writes them.  bfloat16 or float32, head sizes in multiples of 16 up to
         256, at most 64 query heads a key/value head and 8,192 requests and groups.  What lies in pages outside a
-        request's positions does not count, whatever it is.  With bfloat16 and head sizes of 64 and 128 a value of a later token of
-        the same portion that is not finite may reach a token in front of it.
+        request's positions does not count, whatever it is, and what a later token of the same portion holds does not count for
+        the tokens in front of it.  (With bfloat16 and head sizes of 64 and 128 such tokens are computed a second time, one by one, where
+        a later one's value is not finite: 1 us a position.)
         """
         # (few Python operations: a call of few rows takes 8 us on the device)
         ints = (block_table, ctx_len, prefix_len, group_off) if cu_q is None else (block_table, ctx_len, prefix_len, group_off, cu_q)

@@ -300,3 +300,55 @@ def test_scales_of_any_sign(ops, dtype, few):
     case.check(got, sums(case))
     flat = Case(8, 2, 64, 16, groups, dtype, seed=52, scale=0.0)
     flat.check(flat.call(ops), sums(flat))
+
+
+POISON = [float("inf"), -float("inf"), float("nan")]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,portions", [((8, 2, 64), [(5, 3)]),                                    # up to 16 rows
+                                            ((4, 1, 128), [(0, 2), (70, 2)]),
+                                            ((14, 2, 64), [(0, 5), (17, 40), (130, 9)] + ones(3, 200)),
+                                            ((28, 4, 128), [(0, 5), (64, 90), (3, 290)] + ones(*range(12))),
+                                            ((6, 2, 48), [(0, 5), (64, 90)])])
+@pytest.mark.parametrize("poison", POISON)
+def test_a_value_that_is_not_finite_stays_out_of_the_rows_in_front_of_it(ops, heads, portions, dtype, poison):
+    """One or two tokens of every portion have such a value in one column: rows in front of them are as if it were not there,
+    rows from them on have what 64 bits make of it there and nothing of it elsewhere."""
+    case = Case(*heads, 16, [(160, portions)], dtype, seed=61, extra_columns=8)
+    at = [[] for _ in case.requests]
+    for r, (P, own, new) in enumerate(case.requests):
+        if new < 2:
+            continue
+        for token in {new // 2, new - 1}:
+            pos, col, kvh = P + own + token, (7 * r + token) % case.hd, r % case.nkv
+            at[r].append((token, col, kvh))
+            case.v[r][pos, kvh, col] = poison
+            case.values[int(case.table[r, pos // 16]), kvh, pos % 16, col] = poison
+    got = case.call(ops).clone()
+    # what is lost by right, checked and put in order, so that the rest can be checked as ever
+    per = case.nq // case.nkv
+    for r, where in enumerate(at):
+        P, own, new = case.requests[r]
+        for token, col, kvh in where:
+            hit = got[case.cu[r] + token:case.cu[r + 1]].view(-1, case.nkv, per, case.hd)[:, kvh, :, col]
+            assert torch.isnan(hit).all() if poison != poison else (hit == poison).all()
+    finite = case.call(ops, out=torch.full_like(case.out, 7.0))
+    assert torch.equal(finite.isnan(), got.isnan())
+    lost = ~torch.isfinite(got)
+    for r, where in enumerate(at):
+        P, own, new = case.requests[r]
+        for token, col, kvh in where:
+            case.v[r][P + own + token, kvh, col] = 0.0
+            lost[case.cu[r] + token:case.cu[r + 1]].view(-1, case.nkv, per, case.hd)[:, kvh, :, col] = False
+    assert not lost.any()
+    # (a column that is lost by right in some rows is 0 there, and what 64 bits make of it without the value is small: it is
+    # taken from a call in which the value is 0)
+    for r, where in enumerate(at):
+        P, own, new = case.requests[r]
+        for token, col, kvh in where:
+            pos = P + own + token
+            case.values[int(case.table[r, pos // 16]), kvh, pos % 16, col] = 0.0
+    clean = case.call(ops, out=torch.full_like(case.out, 7.0))
+    case.check(torch.where(torch.isfinite(got), got, clean), sums(case))
+    ops.check_errors()
