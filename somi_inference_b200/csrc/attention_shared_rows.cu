@@ -10,7 +10,8 @@
 // `mma.sync` m16n8k16 from registers and ldmatrix, with a maximum, a sum and 16 rows of output of its
 // own, so nothing but the ends of pieces is common to the warps.  Three CTAs an SM (192 KB in flight) keep
 // HBM busy across the beginnings and ends of pieces.  Keys outside the piece are not read: cp.async fills zeros.
-// Measured: 2 requests behind 176 positions (14 heads of 64) 7.0 us, behind 8,192 (28 of 128, 17 MB) 17.5: the merge's reading of a
+// Measured (the device's time in a graph of calls; an eager call takes the host 16): 2 requests behind 176 positions (14 heads of 64) 6.9 us, behind
+// 8,192 (28 of 128, 17 MB) 17.5: the merge's reading of a
 // part from every third CTA, the ranges and the hand-over between two kernels, not HBM.
 #include "mma.cuh"
 #include "shared_prefix.cuh"

@@ -26,8 +26,9 @@
 // of the first and last tile before they announce the probabilities.  Every wait on an mbarrier is
 // bounded and failure is recorded in an error word.
 //
-// Measured (28 heads of 128 over 4, in a row): 64 requests behind 8,192 positions with 200 of their own 35.2 us, 8 behind 2,048
-// 13.3, portions of 1 to 47 tokens of 24 requests behind 20,000 163 us (925 TFLOP/s).  Long pieces are bound by the softmax
+// Measured (28 heads of 128 over 4), the device's time in a graph of calls: 64 requests behind 8,192 positions with up to 511 of their
+// own 35.1 us, 8 behind 2,048 13.2, portions of 1 to 47 tokens of 24 requests behind 20,000 164 us (920 TFLOP/s); as calls one behind
+// the other 35.4, 16.3 (the host's time) and 181 us (830 TFLOP/s).  Long pieces are bound by the softmax
 // chain of a tile (load, maximum, 2^x, store: 2.1 us a pair of tiles), short ones by the chain from the block table to the
 // written part (4.5 us, of which the products are a tenth).
 #include "shared_prefix.cuh"
@@ -39,7 +40,9 @@ namespace shp {
 constexpr int kTcThreads = 384, kTile = 128;          // rows of a warp group; keys of a tile
 constexpr int kTcBlockRows = 2 * kTile;
 // An item of more than 128 rows gathers 256 rows of queries and writes 256 of outputs, and often comes between pieces of the other way:
-// with a cost of 3 beside its units, where one of few rows has 1, 24 portions of 1 to 47 tokens behind 20,000 positions took 157 us (1: 278).
+// with a cost of 3 beside its units, where one of few rows has 1, 24 portions of 1 to 47 tokens behind 20,000 positions take 184 us (1: 278,
+// 2: 213, 4: 166, 6: 169; lengths drawn anew), 16 of 100 behind 4,096 148 (1: 232, 2: 177, 4: 143, 6: 148), 60 of 1 to 20 behind 2,000
+// 55.1 (58.7, 56.4, 61.2, 60.8), 8 of 60 behind 1,024 36.0 (38.1, 37.7, 36.9, 38.5); single tokens differ by 0.6 at most.
 constexpr int kOverWide = 3;
 constexpr int kPieces = 4;                            // of the ring of pieces
 constexpr int kHalf = kTile * 128;                    // bytes of a [128][64] swizzled block

@@ -30,8 +30,8 @@
 // weights are computed a second time to find where the numbers fall (where top-p's bin was sorted, the bins above it tell every CTA
 // what it keeps, and only one on which a number falls weighs again).
 //
-// Measured (152,064 logits): 1 row with all filters 10.8 us (a chain of exchanges and a sort; HBM would need 0.1), 8 rows without
-// any 13.2, 64 rows of mixed settings 57.6 (about 90 instructions a weight and token), 256 bfloat16 rows with top-p 217 (weighed once a
+// Measured (152,064 logits): 1 row with all filters 11.1 us (a chain of exchanges and a sort; HBM would need 0.1), 8 rows without
+// any 13.6, 64 rows of mixed settings 61 (57.5 in a graph; about 90 instructions a weight and token), 256 bfloat16 rows with top-p 217 (weighed once a
 // value, 281 once a token): instructions at 2.1 of 4 issue slots a cycle, and barriers.
 #include <cooperative_groups.h>
 
@@ -944,8 +944,10 @@ int launch_draw(const void* logits, long long stride, int rows, int V, const Set
                 int* out, float* prob, cudaStream_t stream) {
     int ranks = 1;
     const auto bytes_of = [&](int n) { return static_cast<long long>(V) / n * static_cast<long long>(sizeof(T)); };
-    // (16 CTAs a row while the rows' clusters find room beside each other: 152,064 logits with top-k, top-p and min-p, 1 row 11.7 us,
-    // with 8 13.1; 12 rows 14.4 and 15.8; 16 rows 20.5 and 16.5)
+    // (16 CTAs a row while the rows' clusters find room beside each other.  152,064 float32 logits, 16 CTAs and 8: without filters 1 row
+    // 9.2 us and 13.3, 8 rows 13.1 and 14.8, 12 rows 13.2 and 19.1, 16 rows 19.4 and 20.1, 24 rows 24.3 and 20.3; with top-p alone 31 and 42,
+    // 41 and 46, 44 and 55, 59 and 54, 71 and 57; with top-k 50 11.3 and 12.8, 15.6 and 14.0, 14.9 and 15.7, 20.6 and 16.5, 22.7 and 17.2;
+    // bfloat16 the same within a microsecond but for top-p, 12 rows 46.1 and 44.8.  32,000 logits take eight in any case.)
     while (ranks < (rows <= 12 ? kMaxCluster : 8) && V > ranks * 4096 && !(rows * ranks >= 256 && bytes_of(ranks) <= 78 * 1024)) ranks *= 2;
     const auto segment = [&](int n) { return ((V + n * kWarps - 1) / (n * kWarps) + 7) / 8 * 8; };
     while (ranks < kMaxCluster && static_cast<long long>(segment(ranks)) * kWarps * sizeof(T) > kMostSlice) ranks *= 2;

@@ -4,7 +4,8 @@ The first four fields, their defaults and their ranges are the reference's
 (somi_inference/core/sampler.py:11-25): temperature >= 0 with 0 meaning greedy
 argmax, top_k == -1 (off) or > 0, top_p in (0, 1], repetition_penalty > 0.
 `min_p` is an addition: tokens with less than `min_p` of the most likely one's probability are left
-out, behind temperature, top-k and top-p; in [0, 1], 0 is off.
+out, behind temperature, top-k and top-p; in [0, 1], 0 is off.  A row with it is drawn by another kernel, which cuts
+exactly `top_k` tokens (equal ones by their index) where the usual one keeps all that equal the k-th.
 `seed` is an addition: the reference draws from the global generator
 (sampler.py:172-173); here every request has its own counter-based stream, so
 its tokens do not depend on what else is in the batch.  None picks a seed at
