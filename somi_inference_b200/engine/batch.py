@@ -49,7 +49,7 @@ LONG_PORTION = 1024
 class PortionFacts(NamedTuple):
     """What a step's multi-token requests have to do with what it shares."""
 
-    saved_bits: int             # as above, of the runs that have such a request among their members
+    saved_bits: int             # as in SharedPrefixes, of the runs that have such a request among their members
     deep: bool                  # one of them continues from DEEP_PORTION cached positions or more, and four times its tokens
     long: bool                  # one of them has more than LONG_PORTION tokens
 
